@@ -60,6 +60,13 @@ SIGNATURES = {
     "i2r_attention_fwd_h2_lse": [P, P, P, I, I, I, P],
     "i2r_attention_bwd_f32": [P, P, P, P, P, P, I, I, I, P],
     "i2r_attention_bwd_h2": [P, P, P, P, P, P, P, I, I, I, P],
+    "i2r_packed_attention_fwd_ws_bytes": [I, I, I, I, I, I, I],
+    "i2r_packed_attention_fwd": [P, P, P, P, P, P, P, P, P, L, I, I, I, I, I, I, L, L, L, L, L, L, F, I, P],
+    "i2r_packed_attention_bwd_ws_bytes": [I, I, I, I, I, I, I, I],
+    "i2r_packed_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, P, P, L, I, I, I, I, I, I, L, L, L, L, L, L, F, P],
+    "i2r_relative_bias_fwd": [P, P, P, P, P, I, I, I, I, I, I, P],
+    "i2r_relative_bias_bwd_ws_bytes": [I, I, I, I],
+    "i2r_relative_bias_bwd": [P, P, P, P, P, P, L, I, I, I, I, I, I, P],
     "i2r_pos_embedding_f32": [P, P, I, I, I, P],
     "i2r_linear_fwd_f32": [P, P, P, P, P, I, I, I, I, P],
     "i2r_linear_bwd_f32": [P, P, P, P, P, P, I, I, I, P],
@@ -83,7 +90,8 @@ SIGNATURES = {
 
 RETURNS_LONG = {"i2r_conv2d_packed_floats", "i2r_conv2d_splitk_floats", "i2r_conv2d_packed_h2_bytes",
                 "i2r_conv2d_splitk_h2_floats", "i2r_conv2d_fwd_h2_noalloc_max_floats",
-                "i2r_conv2d_wgrad_det_floats"}
+                "i2r_conv2d_wgrad_det_floats", "i2r_packed_attention_fwd_ws_bytes",
+                "i2r_packed_attention_bwd_ws_bytes", "i2r_relative_bias_bwd_ws_bytes"}
 
 _lib = None
 

@@ -1,0 +1,203 @@
+// Attention over packed sequences with a bucketed relative position bias: forward and backward.
+#include "packed_rows.h"
+
+#define WAVES 4  // rows a workgroup works on, one wave each
+
+// One wave for each (row, head).
+template <typename T>
+__global__ __launch_bounds__(64 * WAVES) void pa_fwd_rows_kernel(PaArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long item = (long)blockIdx.x * WAVES + (threadIdx.x >> 6);
+  const long slot = item / a.heads;
+  const int h = item % a.heads;
+  if (slot >= (long)a.nq + a.s.batch + 2) return;
+  int start;
+  const int span = pa_span(a.s.cu_q, a.s.batch, a.nq, 0, slot, start);
+  const long row = start + (slot - (long)start - span);
+  if (span == 0 || span > a.s.batch) {
+    const int end = span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq;
+    if (row < end) {
+      const long at = (row * a.heads + h) * a.dim;
+      for (int d = lane; d < a.dim; d += 64) {
+        if (a.zero_outside) ((T*)a.out)[at + d] = (T)0.0f;
+        if (a.out32) a.out32[at + d] = 0.0f;
+      }
+    }
+    return;
+  }
+  const PaSeq w = pa_seq(a.s, a.nq, a.nk, span - 1);
+  if (row >= w.q0 + w.lq) return;
+  pa_row_fwd<T>(a, w, (int)(row - w.q0), h);
+}
+
+// delta = <dout, out> of each row and head
+template <typename T>
+__global__ __launch_bounds__(64 * WAVES) void pa_delta_kernel(PaArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long item = (long)blockIdx.x * WAVES + (threadIdx.x >> 6);
+  if (item >= (long)a.nq * a.heads) return;
+  const long row = item / a.heads, at = item * a.dim;
+  float s = 0.0f;
+  for (int d = lane; d < a.dim; d += 64) s = fmaf((float)((const T*)a.dout)[at + d], a.out32_in[at + d], s);
+  s = wave_sum(s);
+  if (lane == 0) a.delta[(item % a.heads) * a.nq + row] = s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(64 * WAVES) void pa_dq_rows_kernel(PaArgs a) {
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long item = (long)blockIdx.x * WAVES + wave;
+  const long slot = item / a.heads;
+  const int h = item % a.heads, nb = a.part ? a.s.num_buckets : 0;
+  if (slot >= (long)a.nq + a.s.batch + 2) return;
+  float* hist = a.part ? lds + wave * nb * 64 : nullptr;
+  for (int c = 0; c < nb; ++c) hist[c * 64 + lane] = 0.0f;
+  int start;
+  const int span = pa_span(a.s.cu_q, a.s.batch, a.nq, 0, slot, start);
+  const long row = start + (slot - (long)start - span);
+  if (span == 0 || span > a.s.batch) {
+    const int end = span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq;
+    if (row < end && a.dq)
+      for (int d = lane; d < a.dim; d += 64) ((T*)a.dq)[(row * a.heads + h) * a.dim + d] = (T)0.0f;
+  } else {
+    const PaSeq w = pa_seq(a.s, a.nq, a.nk, span - 1);
+    if (row < w.q0 + w.lq) pa_row_dq<T>(a, w, (int)(row - w.q0), h, hist);
+  }
+  for (int c = 0; c < nb; ++c) {
+    const float s = wave_sum(hist[c * 64 + lane]);
+    if (lane == 0) a.part[(slot * a.heads + h) * nb + c] = s;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(64 * WAVES) void pa_dkv_rows_kernel(PaArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long item = (long)blockIdx.x * WAVES + (threadIdx.x >> 6);
+  const long slot = item / a.kv_heads;
+  const int g = item % a.kv_heads;
+  if (slot >= (long)a.nk + a.s.batch + 2) return;
+  int start;
+  const int span = pa_span(a.s.cu_k, a.s.batch, a.nk, 0, slot, start);
+  const long row = start + (slot - (long)start - span);
+  int end = span > a.s.batch ? a.nk : pa_clamp(a.s.cu_k[span], a.nk);
+  if (row >= end) return;
+  PaSeq w = {};
+  if (span > 0 && span <= a.s.batch) w = pa_seq(a.s, a.nq, a.nk, span - 1);
+  if (row - start < w.lk) {
+    pa_row_dkv<T>(a, w, (int)(row - start), g);
+    return;
+  }
+  for (int d = lane; d < a.dim; d += 64) {
+    const long at = (row * a.kv_heads + g) * a.dim + d;
+    ((T*)a.dk)[at] = ((T*)a.dv)[at] = (T)0.0f;
+  }
+}
+
+// dtable[h][c] = sum of the parts, in a fixed order: each thread a stride of them, then a tree
+__global__ __launch_bounds__(256) void pa_dtable_kernel(const float* part, float* dtable, long parts, int heads, int nb) {
+  __shared__ float sum[256];
+  const int h = blockIdx.x, c = blockIdx.y;
+  float s = 0.0f;
+  for (long i = threadIdx.x; i < parts; i += 256) s += part[(i * heads + h) * nb + c];
+  sum[threadIdx.x] = s;
+  for (int n = 128; n > 0; n >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < n) sum[threadIdx.x] += sum[threadIdx.x + n];
+  }
+  if (threadIdx.x == 0) dtable[(long)h * nb + c] = sum[0];
+}
+
+static long esize(int dtype) { return dtype == 0 ? 4 : 2; }
+
+static int check(const char* what, const i2r_packed_seqs* s, const void* q, const void* k, const void* v, const float* table,
+                 int dtype, int nq, int nk, int heads, int kv_heads, int dim, const long (&strides)[6]) {
+  I2R_REQUIRE(s && s->cu_q && s->cu_k && s->batch > 0, "%s: no sequences", what);
+  I2R_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d is not 0 (fp32), 1 (fp16) or 2 (bf16)", what, dtype);
+  I2R_REQUIRE(nq >= 0 && nk >= 0, "%s: negative number of rows", what);
+  I2R_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "%s: %d heads are no multiple of %d key / value heads",
+              what, heads, kv_heads);
+  I2R_REQUIRE(dim >= 8 && dim <= 128 && dim % 8 == 0, "%s: head dim %d is not a multiple of 8 up to 128", what, dim);
+  I2R_REQUIRE((q || !nq) && (k || !nk) && (v || !nk), "%s: null tensor", what);
+  I2R_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: q, k and v have to be 16-byte aligned", what);
+  for (long st : strides)
+    I2R_REQUIRE(st >= 0 && st * esize(dtype) % 16 == 0, "%s: strides have to be whole multiples of 16 bytes", what);
+  I2R_REQUIRE(!s->pos_q == !s->pos_k, "%s: positions of queries and keys come together", what);
+  if (table) {
+    I2R_REQUIRE(s->lut && s->num_buckets > 0 && s->num_buckets <= PA_MAX_BUCKETS, "%s: %d buckets: 1 to %d are supported",
+                what, s->num_buckets, PA_MAX_BUCKETS);
+    I2R_REQUIRE(s->max_distance >= 0 && s->max_distance <= PA_MAX_DISTANCE, "%s: distance %d: 0 to %d are supported", what,
+                s->max_distance, PA_MAX_DISTANCE);
+  }
+  return I2R_OK;
+}
+
+#define PA_DISPATCH(KERNEL, GRID, LDS)                                                               \
+  switch (dtype) {                                                                                   \
+    case 0: hipLaunchKernelGGL(KERNEL<float>, dim3(GRID), dim3(64 * WAVES), LDS, st, a); break;       \
+    case 1: hipLaunchKernelGGL(KERNEL<f16_t>, dim3(GRID), dim3(64 * WAVES), LDS, st, a); break;       \
+    default: hipLaunchKernelGGL(KERNEL<bf16_t>, dim3(GRID), dim3(64 * WAVES), LDS, st, a); break;     \
+  }
+
+extern "C" long i2r_packed_attention_fwd_ws_bytes(int, int, int, int, int, int, int) { return 0; }
+
+extern "C" int i2r_packed_attention_fwd(const i2r_packed_seqs* seqs, const void* q, const void* k, const void* v,
+                                        const float* table, void* out, float* out32, float* stats, void* ws, long ws_bytes,
+                                        int dtype, int nq, int nk, int heads, int kv_heads, int dim, long q_row, long q_head,
+                                        long k_row, long k_head, long v_row, long v_head, float scale, int zero_outside,
+                                        i2r_stream_t stream) {
+  if (int rc = check("packed_attention_fwd", seqs, q, k, v, table, dtype, nq, nk, heads, kv_heads, dim,
+                     {q_row, q_head, k_row, k_head, v_row, v_head}))
+    return rc;
+  if (nq == 0) return I2R_OK;
+  I2R_REQUIRE(out && (uintptr_t)out % 16 == 0, "packed_attention_fwd: out is null or not 16-byte aligned");
+  hipStream_t st = (hipStream_t)stream;
+  PaArgs a = {};
+  a.s = *seqs;
+  a.q = q, a.k = k, a.v = v, a.table = table, a.out = out, a.out32 = out32, a.stats = stats;
+  a.nq = nq, a.nk = nk, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.scale = scale, a.zero_outside = zero_outside;
+  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  const long items = ((long)nq + seqs->batch + 2) * heads;
+  I2R_REQUIRE(items / WAVES < INT32_MAX, "packed_attention_fwd: too many rows");
+  PA_DISPATCH(pa_fwd_rows_kernel, i2r_cdiv(items, WAVES), 0);
+  return i2r_check_launch("packed_attention_fwd");
+}
+
+extern "C" long i2r_packed_attention_bwd_ws_bytes(int, int batch, int nq, int, int heads, int, int, int num_buckets) {
+  return ((long)nq * heads + ((long)nq + batch + 2) * heads * num_buckets) * 4;
+}
+
+extern "C" int i2r_packed_attention_bwd(const i2r_packed_seqs* seqs, const void* q, const void* k, const void* v,
+                                        const float* table, const float* out32, const float* stats, const void* dout,
+                                        void* dq, void* dk, void* dv, float* dtable, void* ws, long ws_bytes, int dtype,
+                                        int nq, int nk, int heads, int kv_heads, int dim, long q_row, long q_head, long k_row,
+                                        long k_head, long v_row, long v_head, float scale, i2r_stream_t stream) {
+  if (int rc = check("packed_attention_bwd", seqs, q, k, v, table, dtype, nq, nk, heads, kv_heads, dim,
+                     {q_row, q_head, k_row, k_head, v_row, v_head}))
+    return rc;
+  I2R_REQUIRE((out32 && stats && dout) || !nq, "packed_attention_bwd: out32, stats and dout are required");
+  I2R_REQUIRE(((uintptr_t)out32 | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0,
+              "packed_attention_bwd: tensors have to be 16-byte aligned");
+  I2R_REQUIRE(!dk == !dv, "packed_attention_bwd: dk and dv come together");
+  I2R_REQUIRE(table || !dtable, "packed_attention_bwd: dtable without a table");
+  const int nb = dtable ? seqs->num_buckets : 0;
+  I2R_REQUIRE(ws_bytes >= i2r_packed_attention_bwd_ws_bytes(dtype, seqs->batch, nq, nk, heads, kv_heads, dim, nb) &&
+                  (ws || !nq),
+              "packed_attention_bwd: workspace too small");
+  hipStream_t st = (hipStream_t)stream;
+  PaArgs a = {};
+  a.s = *seqs;
+  a.q = q, a.k = k, a.v = v, a.table = table, a.out32_in = out32, a.stats = (float*)stats, a.dout = dout;
+  a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)ws, a.part = dtable ? (float*)ws + (long)nq * heads : nullptr;
+  a.nq = nq, a.nk = nk, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.scale = scale;
+  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  const long slots_q = (long)nq + seqs->batch + 2, slots_k = (long)nk + seqs->batch + 2;
+  I2R_REQUIRE(slots_q * heads / WAVES < INT32_MAX && slots_k * kv_heads / WAVES < INT32_MAX,
+              "packed_attention_bwd: too many rows");
+  if (nq) PA_DISPATCH(pa_delta_kernel, i2r_cdiv((long)nq * heads, WAVES), 0);
+  if (dq || dtable) PA_DISPATCH(pa_dq_rows_kernel, i2r_cdiv(slots_q * heads, WAVES), nb * 64 * 4 * WAVES);
+  if (dtable)
+    hipLaunchKernelGGL(pa_dtable_kernel, dim3(heads, nb), dim3(256), 0, st, a.part, dtable, slots_q, heads, nb);
+  if (dk && nk) PA_DISPATCH(pa_dkv_rows_kernel, i2r_cdiv(slots_k * kv_heads, WAVES), 0);
+  return i2r_check_launch("packed_attention_bwd");
+}

@@ -193,6 +193,56 @@ int i2r_attention_bwd_f32(const float* qkv, const float* out, const float* lse, 
 int i2r_attention_bwd_h2(const float* qkv, const float* out, const float* lse, const float* dout, float* dqkv,
                          float* delta_ws, const float* scale, int B, int heads, int T, i2r_stream_t stream);
 
+/* ---- attention over packed sequences, relative position bias by buckets (no counterpart in the reference) ----------- */
+/* Sequences of different lengths lie one behind the other: sequence b owns rows cu_q[b] .. cu_q[b+1] of q and out and
+ * rows cu_k[b] .. cu_k[b+1] of k and v, of which the first len_k[b] hold keys (all of them when len_k is NULL; a cache
+ * with room is cu_k = b * room with len_k its fill).  The arrays are DEVICE int32 and may change between calls; values
+ * outside the tensors are clamped to them.  With `causal` query i of Lq sees keys j <= i + Lk - Lq.
+ * Bias: lut[n] is the bucket of distance n - max_distance (key position less query position, clamped to
+ * +-max_distance); positions are pos_k[row], pos_q[row], or without them j and i + Lk - Lq within the sequence. */
+typedef struct i2r_packed_seqs {
+  const int* cu_q;            /* batch + 1 */
+  const int* cu_k;            /* batch + 1 */
+  const int* len_k;           /* batch, or NULL */
+  const int* pos_q;           /* a position for each row of q, or NULL (then pos_k is NULL too) */
+  const int* pos_k;           /* a position for each row of k */
+  const unsigned char* lut;   /* 2 * max_distance + 1 bucket numbers < num_buckets; NULL without a bias */
+  int batch, causal, num_buckets /* <= 64 */, max_distance /* <= 1024 */;
+} i2r_packed_seqs;
+/* out_i = sum_j softmax_j(scale * <q_i, k_j> + table[h][bucket]) v_j for each query head h and its key / value head
+ * h / (heads / kv_heads).  dtype: 0 fp32, 1 fp16, 2 bf16 (q, k, v, out alike); dim a multiple of 8 up to 128; each row of
+ * q, k, v: `dim` contiguous elements, token and head strides in ELEMENTS, rows 16-byte aligned; out (nq, heads, dim)
+ * contiguous.  A query that sees no key, or only scores of -inf, gets 0.  Hidden keys' values are never used, be they
+ * NaN.  table: (heads, num_buckets) fp32 or NULL.  stats (2 * heads * nq floats: per row the softmax's reference exponent
+ * and log2 of its sum) and out32 (out before its rounding; NULL for fp32) are what the backward reads; NULL when there is
+ * none.  zero_outside: rows of no sequence are zeroed in out (0: left as they were).  ws: ws_bytes from the query (may be
+ * 0: then NULL). */
+long i2r_packed_attention_fwd_ws_bytes(int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dim);
+int i2r_packed_attention_fwd(const i2r_packed_seqs* seqs, const void* q, const void* k, const void* v,
+                             const float* table, void* out, float* out32, float* stats, void* ws, long ws_bytes,
+                             int dtype, int nq, int nk, int heads, int kv_heads, int dim, long q_row, long q_head,
+                             long k_row, long k_head, long v_row, long v_head, float scale, int zero_outside,
+                             i2r_stream_t stream);
+/* Gradients, all contiguous: dq (nq, heads, dim), dk, dv (nk, kv_heads, dim), dtable (heads, num_buckets) fp32; any may be
+ * NULL (dk and dv together).  out32: the forward's out32 (fp32: its out).  dout contiguous.  Rows of no sequence and
+ * rows behind a sequence's keys get 0.  Every sum has a fixed order: the same inputs give the same bits. */
+long i2r_packed_attention_bwd_ws_bytes(int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dim,
+                                       int num_buckets);
+int i2r_packed_attention_bwd(const i2r_packed_seqs* seqs, const void* q, const void* k, const void* v,
+                             const float* table, const float* out32, const float* stats, const void* dout, void* dq,
+                             void* dk, void* dv, float* dtable, void* ws, long ws_bytes, int dtype, int nq, int nk,
+                             int heads, int kv_heads, int dim, long q_row, long q_head, long k_row, long k_head,
+                             long v_row, long v_head, float scale, i2r_stream_t stream);
+/* The bias alone: out (heads, nq, nk) = table[h][lut[pos_k[j] - pos_q[i]]] in `dtype`; positions NULL: j and i + nk - nq.
+ * Backward: dtable (heads, num_buckets) = sums of dout over each bucket's places, in a fixed order. */
+int i2r_relative_bias_fwd(const float* table, const unsigned char* lut, const int* pos_q, const int* pos_k, void* out,
+                          int dtype, int heads, int nq, int nk, int num_buckets, int max_distance,
+                          i2r_stream_t stream);
+long i2r_relative_bias_bwd_ws_bytes(int heads, int nq, int nk, int num_buckets);
+int i2r_relative_bias_bwd(const void* dout, const unsigned char* lut, const int* pos_q, const int* pos_k, float* dtable,
+                          void* ws, long ws_bytes, int dtype, int heads, int nq, int nk, int num_buckets,
+                          int max_distance, i2r_stream_t stream);
+
 /* ---- embedding path: models/networks.py:200-206 (PositionalEmbedding), :39-43 (Linear) ---------------------------- */
 int i2r_pos_embedding_f32(const float* x, float* out, int B, int num_channels, int max_positions,
                           i2r_stream_t stream);
