@@ -1,34 +1,9 @@
 // Attention over packed sequences with a bucketed relative position bias: forward and backward.
 #include "packed_rows.h"
 
-#define WAVES 4  // rows a workgroup works on, one wave each
+bool pa_launch_fwd(int dtype, const PaArgs& a, hipStream_t st);  // packed_fwd.hip
 
-// One wave for each (row, head).
-template <typename T>
-__global__ __launch_bounds__(64 * WAVES) void pa_fwd_rows_kernel(PaArgs a) {
-  const int lane = threadIdx.x & 63;
-  const long item = (long)blockIdx.x * WAVES + (threadIdx.x >> 6);
-  const long slot = item / a.heads;
-  const int h = item % a.heads;
-  if (slot >= (long)a.nq + a.s.batch + 2) return;
-  int start;
-  const int span = pa_span(a.s.cu_q, a.s.batch, a.nq, 0, slot, start);
-  const long row = start + (slot - (long)start - span);
-  if (span == 0 || span > a.s.batch) {
-    const int end = span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq;
-    if (row < end) {
-      const long at = (row * a.heads + h) * a.dim;
-      for (int d = lane; d < a.dim; d += 64) {
-        if (a.zero_outside) ((T*)a.out)[at + d] = (T)0.0f;
-        if (a.out32) a.out32[at + d] = 0.0f;
-      }
-    }
-    return;
-  }
-  const PaSeq w = pa_seq(a.s, a.nq, a.nk, span - 1);
-  if (row >= w.q0 + w.lq) return;
-  pa_row_fwd<T>(a, w, (int)(row - w.q0), h);
-}
+#define WAVES 4  // rows a workgroup works on, one wave each
 
 // delta = <dout, out> of each row and head
 template <typename T>
@@ -114,14 +89,15 @@ static int check(const char* what, const i2r_packed_seqs* s, const void* q, cons
                  int dtype, int nq, int nk, int heads, int kv_heads, int dim, const long (&strides)[6]) {
   I2R_REQUIRE(s && s->cu_q && s->cu_k && s->batch > 0, "%s: no sequences", what);
   I2R_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d is not 0 (fp32), 1 (fp16) or 2 (bf16)", what, dtype);
-  I2R_REQUIRE(nq >= 0 && nk >= 0, "%s: negative number of rows", what);
-  I2R_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "%s: %d heads are no multiple of %d key / value heads",
+  I2R_REQUIRE(nq >= 0 && nk >= 0 && nq < 1 << 30 && nk < 1 << 30, "%s: 0 to 2^30 - 1 rows are supported", what);
+  I2R_REQUIRE(kv_heads > 0 && heads > 0 && heads < 65536 && heads % kv_heads == 0, "%s: %d heads are no multiple of %d key / value heads",
               what, heads, kv_heads);
   I2R_REQUIRE(dim >= 8 && dim <= 128 && dim % 8 == 0, "%s: head dim %d is not a multiple of 8 up to 128", what, dim);
   I2R_REQUIRE((q || !nq) && (k || !nk) && (v || !nk), "%s: null tensor", what);
   I2R_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: q, k and v have to be 16-byte aligned", what);
   for (long st : strides)
-    I2R_REQUIRE(st >= 0 && st * esize(dtype) % 16 == 0, "%s: strides have to be whole multiples of 16 bytes", what);
+    I2R_REQUIRE(st >= 0 && st < 1 << 22 && st * esize(dtype) % 16 == 0,
+                "%s: strides have to be whole multiples of 16 bytes and below 2^22 elements", what);
   I2R_REQUIRE(!s->pos_q == !s->pos_k, "%s: positions of queries and keys come together", what);
   if (table) {
     I2R_REQUIRE(s->lut && s->num_buckets > 0 && s->num_buckets <= PA_MAX_BUCKETS, "%s: %d buckets: 1 to %d are supported",
@@ -157,9 +133,7 @@ extern "C" int i2r_packed_attention_fwd(const i2r_packed_seqs* seqs, const void*
   a.q = q, a.k = k, a.v = v, a.table = table, a.out = out, a.out32 = out32, a.stats = stats;
   a.nq = nq, a.nk = nk, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.scale = scale, a.zero_outside = zero_outside;
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  const long items = ((long)nq + seqs->batch + 2) * heads;
-  I2R_REQUIRE(items / WAVES < INT32_MAX, "packed_attention_fwd: too many rows");
-  PA_DISPATCH(pa_fwd_rows_kernel, i2r_cdiv(items, WAVES), 0);
+  if (!pa_launch_fwd(dtype, a, st)) return I2R_ERR_HIP;
   return i2r_check_launch("packed_attention_fwd");
 }
 

@@ -1,0 +1,220 @@
+// Forward of packed-sequence attention on the matrix cores.
+#include "packed_tiles.h"
+
+// One workgroup: 4 waves x 32 queries of one sequence and head; keys come in tiles of KEYS, the next tile loading while
+// this one is worked on (two LDS buffers, one barrier a tile).
+template <typename T, int DP>
+struct FwdShape {
+  static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
+  typedef Tile<T, DP, KEYS> Tl;
+  static constexpr int BUFFER = 2 * Tl::BYTES + KEYS * 4;  // k, v, positions
+  static int lds(bool bias, int max_distance) { return 2 * BUFFER + (bias ? (2 * max_distance + 1) * 4 : 0); }
+};
+
+// order of the tiles: each of the 8 XCDs (workgroups go to them in turn) works through whole heads, so that a head's keys
+// and values stay in that XCD's L2; within a head the last -- with a causal mask longest -- tiles first
+__device__ __forceinline__ bool tile_of(long slots, int heads, long& slot, int& h) {
+  const long per = (slots * heads + 7) / 8, w = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (w >= slots * heads || (long)(blockIdx.x >> 3) >= per) return false;
+  h = (int)(w / slots);
+  slot = slots - 1 - w % slots;
+  return true;
+}
+
+template <typename T, int DP, bool BIAS, bool SAVE>
+__global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
+  typedef FwdShape<T, DP> S;
+  typedef typename S::Tl Tl;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  long slot;
+  int h, start;
+  if (!tile_of(slots, a.heads, slot, h)) return;
+  const int span = pa_span(a.s.cu_q, a.s.batch, a.nq, 7, slot, start);
+  const long row0 = start + ((slot - (start >> 7) - span) << 7);
+  if (span == 0 || span > a.s.batch) {  // rows of no sequence
+    const int end = (int)min(row0 + S::ROWS, (long)(span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq));
+    for (long i = (row0 * a.dim) + threadIdx.x; i < (long)end * a.dim; i += 256) {
+      const long at = (i / a.dim * a.heads + h) * a.dim + i % a.dim;
+      if (a.zero_outside) ((T*)a.out)[at] = (T)0.0f;
+      if (a.out32) a.out32[at] = 0.0f;
+    }
+    return;
+  }
+  const PaSeq w = pa_seq(a.s, a.nq, a.nk, span - 1);
+  if (row0 >= w.q0 + w.lq) return;
+  const int g = h / (a.heads / a.kv_heads);
+  const int i0 = (int)(row0 - w.q0), iw = i0 + wave * 32, i = iw + col;  // first query of workgroup, wave; lane's own
+  const bool valid = i < w.lq;
+  const int ahead = w.lk - w.lq;  // keys before the query's own
+  int keys = w.lk;                // keys that the workgroup's last query sees
+  if (a.s.causal) keys = min(keys, min(i0 + S::ROWS, w.lq) + ahead);
+
+  Loader<T, DP, S::KEYS, S::WAVES> lk, lv;
+  lk.init((const T*)a.k + (long)w.k0 * a.k_row + g * a.k_head, a.k_row, a.dim);
+  lv.init((const T*)a.v + (long)w.k0 * a.v_row + g * a.v_head, a.v_row, a.dim);
+  float* by_distance = (float*)(lds + 2 * S::BUFFER);
+  const int far = a.s.max_distance;
+  auto load = [&](int n) {
+    char* b = lds + (n & 1) * S::BUFFER;
+    lk.load(b, n * S::KEYS, keys);
+    lv.load(b + Tl::BYTES, n * S::KEYS, keys);
+    if (BIAS && a.s.pos_k && threadIdx.x < S::KEYS) {
+      const int j = n * S::KEYS + threadIdx.x;
+      ((int*)(b + 2 * Tl::BYTES))[threadIdx.x] = j < keys ? a.s.pos_k[w.k0 + j] : 0;
+    }
+  };
+  const int tiles = keys > 0 ? (keys + S::KEYS - 1) / S::KEYS : 0;
+  if (tiles > 0) load(0);
+
+  // a negative scale flips q's sign (exact), so that the largest product is the largest score
+  const float sc = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * PA_LOG2E;
+  frag_t<T> q[Tl::STEPS];
+  load_rows<T>(q, (const T*)a.q + (long)(w.q0 + i) * a.q_row + h * a.q_head, valid && a.scale != 0.0f, a.dim, half);
+  if (a.scale < 0.0f)
+#pragma unroll
+    for (int s = 0; s < Tl::STEPS; ++s) q[s] = -q[s];
+  if (BIAS) load_table(by_distance, a.s, a.table, h);
+  const int pos_q = BIAS && valid ? pa_pos_q(a.s, w, i) : 0;
+
+  f32x16 o[Tl::BLOCKS];
+#pragma unroll
+  for (int b = 0; b < Tl::BLOCKS; ++b) o[b] = (f32x16)0.0f;
+  float m = -INFINITY, l = 0.0f;  // the column's reference exponent; the lane's half of the sum
+
+  for (int n = 0; n < tiles; ++n) {
+    tiles_ready();
+    if (n + 1 < tiles) load(n + 1);
+    const char* kt = lds + (n & 1) * S::BUFFER;
+    const char* vt = kt + Tl::BYTES;
+    const int j0 = n * S::KEYS;
+    if (iw >= w.lq || (a.s.causal && j0 > iw + 31 + ahead)) continue;  // nothing for this wave
+#pragma unroll
+    for (int kb = 0; kb < S::KEYS / 32; ++kb) {
+      const int jb = j0 + kb * 32;
+      f32x16 x = (f32x16)0.0f;
+#pragma unroll
+      for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(kt, kb * 32 + col, s, half), q[s]);
+      if (BIAS) {
+        const int lo = jb - (iw + 31 + ahead), hi = jb + 31 - (iw + ahead);  // smallest and largest distance
+        if (!a.s.pos_q && (hi <= -far || lo >= far)) {
+          const float b = by_distance[hi <= -far ? 0 : 2 * far];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], sc, b);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int row = acc_row(r, half);
+            const int pos_k = a.s.pos_k ? ((const int*)(vt + Tl::BYTES))[kb * 32 + row] : jb + row;
+            x[r] = fmaf(x[r], sc, by_distance[pa_entry(pa_apart(pos_k, pos_q), far)]);
+          }
+        }
+      }
+      const int last = a.s.causal ? min(keys, i + ahead + 1) : keys;  // keys the lane's query sees
+      if (jb + 32 > keys || (a.s.causal && jb + 31 > iw + ahead)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = jb + acc_row(r, half) < last ? x[r] : -INFINITY;
+      }
+      float top = x[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+      top = fmaxf(top, other_half(top));
+      if (!BIAS) top *= sc;
+      // The reference exponent moves only when a score passes it by 2^8: the sums stay far from overflow, and most
+      // blocks rescale nothing.
+      if (__any(top > m + 8.0f || m == -INFINITY)) {
+        const float mn = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= fall;
+#pragma unroll
+        for (int b = 0; b < Tl::BLOCKS; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[b][r] *= fall;
+        m = mn;
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        x[r] = __builtin_amdgcn_exp2f(BIAS ? x[r] - ref : fmaf(x[r], sc, -ref));
+        l += x[r];
+      }
+      // Rounding the probabilities to the type puts each off by at most half a step, independently: as much as rounding
+      // the output once more.  The table's gradient is fp32, and delta = <dout, out> enters it: with a bias to train
+      // the rounded-away rest is multiplied too.
+      Probs<T> p;
+      p.set(x);
+#pragma unroll
+      for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(vt, kb * 32, b, lane, p, o[b]);
+      if constexpr (BIAS && SAVE && sizeof(T) == 2) {
+        Probs<T> rest;
+        rest.set_rest(x, p);
+#pragma unroll
+        for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(vt, kb * 32, b, lane, rest, o[b]);
+      }
+    }
+  }
+
+  l += other_half(l);
+  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  float finite = l * 0.0f;
+  const long at = ((long)(w.q0 + i) * a.heads + h) * a.dim;
+#pragma unroll
+  for (int b = 0; b < Tl::BLOCKS; ++b)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int d = b * 32 + 8 * t + 4 * half;
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      t4 y;
+      f32x4 z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        z[e] = o[b][4 * t + e] * inv;
+        finite = fmaf(z[e], 0.0f, finite);
+        y[e] = (T)z[e];
+      }
+      if (valid && d < a.dim) {
+        *(t4*)((T*)a.out + at + d) = y;
+        if (SAVE && sizeof(T) == 2 && a.out32) *(f32x4*)(a.out32 + at + d) = z;
+      }
+    }
+  if (SAVE && valid && half == 0) {
+    a.stats[(long)h * a.nq + w.q0 + i] = m == -INFINITY ? 0.0f : m;
+    a.stats[(long)(a.heads + h) * a.nq + w.q0 + i] = m == -INFINITY ? INFINITY : log2f(l);
+  }
+  // A product of a hidden key's probability 0 with an infinity or NaN is NaN: rows that came out so are done again, pair
+  // by pair, without the hidden ones.
+  unsigned long long again = __ballot(valid && !(finite == 0.0f));
+  for (unsigned rows = (unsigned)again | (unsigned)(again >> 32); rows; rows &= rows - 1)
+    pa_row_fwd<T>(a, w, iw + __ffs(rows) - 1, h);
+}
+
+template <typename T, int DP>
+static void launch_fwd(const PaArgs& a, hipStream_t st, bool& ok) {
+  typedef FwdShape<T, DP> S;
+  const bool bias = a.table != nullptr, save = a.stats != nullptr;
+  const long slots = (a.nq >> 7) + a.s.batch + 2;
+  const int lds = S::lds(bias, a.s.max_distance);
+  const dim3 grid((unsigned)((slots * a.heads + 7) / 8 * 8));
+#define PA_FWD(B, V)                                                                                \
+  {                                                                                                 \
+    static bool done[64];                                                                           \
+    ok = i2r_lds_attr((const void*)pa_fwd_kernel<T, DP, B, V>, S::lds(true, PA_MAX_DISTANCE), done); \
+    if (ok) hipLaunchKernelGGL((pa_fwd_kernel<T, DP, B, V>), grid, dim3(256), lds, st, a, slots);   \
+  }
+  if (bias && save) PA_FWD(true, true)
+  else if (bias) PA_FWD(true, false)
+  else if (save) PA_FWD(false, true)
+  else PA_FWD(false, false)
+}
+
+bool pa_launch_fwd(int dtype, const PaArgs& a, hipStream_t st) {
+  bool ok = true;
+  const int dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
+#define PA_BY_DIM(T)                          \
+  if (dp == 32) launch_fwd<T, 32>(a, st, ok); \
+  else if (dp == 64) launch_fwd<T, 64>(a, st, ok); \
+  else launch_fwd<T, 128>(a, st, ok);
+  if (dtype == 0) { PA_BY_DIM(float) }
+  else if (dtype == 1) { PA_BY_DIM(f16_t) }
+  else { PA_BY_DIM(bf16_t) }
+  return ok;
+}

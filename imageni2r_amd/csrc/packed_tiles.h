@@ -1,0 +1,180 @@
+// Tiles of packed sequences on the matrix cores.
+//
+// Every product here has a 32-column operand B in registers (a column is a query row in the forward and dq kernels, a key
+// in the dk / dv kernel) and its other operand A in a 32-row block of an LDS tile, so that a lane's 16 accumulators belong
+// to ONE column: softmax statistics, masks and rescaling are per lane, and the accumulators of the first product, rounded
+// to the type, ARE the second product's B operand -- they never pass through LDS or another lane.  That works because the
+// order of the contracted index is free: accumulator r of lane half h belongs to row (r & 3) + 8 * (r >> 2) + 4 * h of its
+// block, and A's transposed fragments are read from LDS in that same order.
+#pragma once
+#include "packed_rows.h"
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+#define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
+
+// row of the block that accumulator r of lane half h holds
+__device__ __forceinline__ constexpr int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+// 16 bytes of a row: the A or B operand of one step (32 bytes of a row, half h of the lanes the h-th 16)
+template <typename T>
+struct Frag {
+  typedef T type __attribute__((ext_vector_type(16 / sizeof(T))));
+};
+template <typename T>
+using frag_t = typename Frag<T>::type;
+
+__device__ __forceinline__ void mma_step(f32x16& c, frag_t<bf16_t> a, frag_t<bf16_t> b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_step(f32x16& c, frag_t<f16_t> a, frag_t<f16_t> b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_step(f32x16& c, frag_t<float> a, frag_t<float> b) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+}
+
+// A tile of ROWS rows of DP elements (the head dim padded with zeros), 16-byte chunks of a row exchanged by its number so
+// that the 32 rows of a fragment read, and the 4 x 64 bytes of a transposed one, fall on different banks.
+template <typename T, int DP, int ROWS>
+struct Tile {
+  static constexpr int ROW_BYTES = DP * (int)sizeof(T), CHUNKS = ROW_BYTES / 16, BYTES = ROWS * ROW_BYTES;
+  static constexpr int STEPS = ROW_BYTES / 32;  // steps of a product over the head dim
+  static constexpr int BLOCKS = DP / 32;        // 32-wide blocks of the head dim
+
+  __device__ static __forceinline__ int swizzle(int row) {
+    return CHUNKS >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : CHUNKS == 8 ? ((row & 1) << 2) | ((row >> 1) & 3) : (row >> 1) & 3;
+  }
+  __device__ static __forceinline__ int at(int row, int chunk) { return row * ROW_BYTES + ((chunk ^ swizzle(row)) << 4); }
+
+  // fragment of row `row` (the lane's own) for step s
+  __device__ static __forceinline__ frag_t<T> frag(const char* tile, int row, int s, int h) {
+    return *(const frag_t<T>*)(tile + at(row, 2 * s + h));
+  }
+
+  // acc[32 d of block db][columns] += tile(rows r0 .. r0 + 32)^T p, p the accumulators of those rows
+  template <typename P>
+  __device__ static __forceinline__ void mma_t(const char* tile, int r0, int db, int lane, const P& p, f32x16& acc) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = db * 32 + (lane & 31), row = r0 + acc_row(r, h);
+        const float a = *(const float*)(tile + at(row, d >> 2) + (d & 3) * 4);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc, 0, 0, 0);
+      }
+    } else {
+      // ds_read_b64_tr_b16: of each 16 lanes, lane t addresses 4 elements of row t >> 2, and gets column t of the 4 rows
+      const int t = lane & 15, row = r0 + 4 * h + (t >> 2);
+      const int chunk = db * 4 + ((lane >> 4) & 1) * 2 + ((t & 3) >> 1);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            LDS_PTR(s16x4, (char*)tile + at(row + 16 * c, chunk) + (t & 1) * 8));
+        s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            LDS_PTR(s16x4, (char*)tile + at(row + 16 * c + 8, chunk) + (t & 1) * 8));
+        const s16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        mma_step(acc, __builtin_bit_cast(frag_t<T>, a), p[c]);
+      }
+    }
+  }
+};
+
+// The accumulators of a 32-row block as B operands: two fragments of 8 in the 16-bit types, the accumulators in fp32.
+template <typename T>
+struct Probs {
+  frag_t<T> f[2];
+  __device__ __forceinline__ const frag_t<T>& operator[](int c) const { return f[c]; }
+  __device__ __forceinline__ void set(const f32x16& x) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) f[r >> 3][r & 7] = (T)x[r];
+  }
+  // what set() rounded away
+  __device__ __forceinline__ void set_rest(const f32x16& x, const Probs& first) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) f[r >> 3][r & 7] = (T)(x[r] - (float)first.f[r >> 3][r & 7]);
+  }
+};
+template <>
+struct Probs<float> {
+  f32x16 f;
+  __device__ __forceinline__ float operator[](int r) const { return f[r]; }
+  __device__ __forceinline__ void set(const f32x16& x) { f = x; }
+};
+
+// Loads tiles of rows of one (sequence, head) into LDS without passing through registers.  Rows behind the last and
+// columns behind the head dim are out of the descriptor's range and arrive as zeros.
+template <typename T, int DP, int ROWS, int WAVES>
+struct Loader {
+  typedef Tile<T, DP, ROWS> Tl;
+  static constexpr int LOADS = Tl::BYTES / (1024 * WAVES);  // 1 KiB for each wave and instruction
+  static_assert(LOADS * 1024 * WAVES == Tl::BYTES, "a tile has to be whole instructions of all waves");
+  const char* base;
+  long step;   // bytes from one row to the next
+  int width;   // bytes of a row that hold elements
+  int offset[LOADS];
+
+  __device__ __forceinline__ void init(const T* p, long row_stride, int dim) {
+    base = (const char*)p, step = row_stride * (long)sizeof(T), width = dim * (int)sizeof(T);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int chunk = (i * WAVES + wave) * 64 + lane, row = chunk / Tl::CHUNKS;
+      const int c = (chunk % Tl::CHUNKS) ^ Tl::swizzle(row);
+      offset[i] = c * 16 < width ? (int)(row * step) + c * 16 : 0x7fffffff;
+    }
+  }
+  // rows first .. first + ROWS of `rows` into the tile (in flight until the next tiles_ready()).
+  // Written out, not by builtin: the compiler would wait for these loads before it reads any other part of LDS.
+  __device__ __forceinline__ void load(char* tile, int first, int rows) const {
+    const int left = min(rows - first, ROWS);
+    const unsigned long long at = (unsigned long long)(base + (long)first * step);
+    i32x4 rs;
+    rs[0] = __builtin_amdgcn_readfirstlane((int)at);
+    rs[1] = __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff);
+    rs[2] = __builtin_amdgcn_readfirstlane(left > 0 ? (int)((left - 1) * step) + width : 0);
+    rs[3] = 0x00020000;
+    const int to = __builtin_amdgcn_readfirstlane((int)(unsigned long)LDS_PTR(char, tile) + (threadIdx.x >> 6) * 1024);
+    asm volatile("s_nop 4" : : "s"(rs), "s"(to));  // a vector instruction may have written them just before
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :
+                   : "s"(to + i * WAVES * 1024), "v"(offset[i]), "s"(rs)
+                   : "memory");
+  }
+};
+
+// B operand of 32 rows, straight from memory: lane's row, zeros where it does not exist
+template <typename T, int STEPS>
+__device__ __forceinline__ void load_rows(frag_t<T> (&f)[STEPS], const T* row, bool valid, int dim, int h) {
+  constexpr int N = 16 / sizeof(T);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int d = (2 * s + h) * N;
+    f[s] = (frag_t<T>)(T)0.0f;
+    if (valid && d < dim) f[s] = *(const frag_t<T>*)(row + d);
+  }
+}
+
+// the value of the lane with the other half of the same column
+__device__ __forceinline__ float other_half(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// workgroup barrier after which the tiles that all waves have asked for are in LDS
+__device__ __forceinline__ void tiles_ready() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The table of one head by distance, in log2 units, and the bucket numbers beside it.
+__device__ __forceinline__ void load_table(float* by_distance, const i2r_packed_seqs& s, const float* table, int h) {
+  for (int n = threadIdx.x; n <= 2 * s.max_distance; n += blockDim.x)
+    by_distance[n] = pa_log2_units(table[(long)h * s.num_buckets + min((int)s.lut[n], s.num_buckets - 1)]);
+}

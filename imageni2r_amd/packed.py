@@ -147,7 +147,7 @@ def _rows(t, name, dtype, device):
     if t.device != device:
         raise ValueError(f"{name}: on {t.device}, the sequences on {device}")
     s0, s1, s2 = t.stride()
-    if s2 != 1 or (s0 * t.element_size()) % 16 or (s1 * t.element_size()) % 16 or t.data_ptr() % 16:
+    if s2 != 1 or (s0 * t.element_size()) % 16 or (s1 * t.element_size()) % 16 or t.data_ptr() % 16 or max(s0, s1) >= 1 << 22:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
