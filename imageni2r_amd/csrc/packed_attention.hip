@@ -2,6 +2,7 @@
 #include "packed_rows.h"
 
 bool pa_launch_fwd(int dtype, const PaArgs& a, hipStream_t st);  // packed_fwd.hip
+bool pa_launch_bwd(int dtype, const PaArgs& a, hipStream_t st, bool dq, bool dkv);  // packed_bwd.hip
 
 #define WAVES 4  // rows a workgroup works on, one wave each
 
@@ -16,57 +17,6 @@ __global__ __launch_bounds__(64 * WAVES) void pa_delta_kernel(PaArgs a) {
   for (int d = lane; d < a.dim; d += 64) s = fmaf((float)((const T*)a.dout)[at + d], a.out32_in[at + d], s);
   s = wave_sum(s);
   if (lane == 0) a.delta[(item % a.heads) * a.nq + row] = s;
-}
-
-template <typename T>
-__global__ __launch_bounds__(64 * WAVES) void pa_dq_rows_kernel(PaArgs a) {
-  extern __shared__ float lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long item = (long)blockIdx.x * WAVES + wave;
-  const long slot = item / a.heads;
-  const int h = item % a.heads, nb = a.part ? a.s.num_buckets : 0;
-  if (slot >= (long)a.nq + a.s.batch + 2) return;
-  float* hist = a.part ? lds + wave * nb * 64 : nullptr;
-  for (int c = 0; c < nb; ++c) hist[c * 64 + lane] = 0.0f;
-  int start;
-  const int span = pa_span(a.s.cu_q, a.s.batch, a.nq, 0, slot, start);
-  const long row = start + (slot - (long)start - span);
-  if (span == 0 || span > a.s.batch) {
-    const int end = span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq;
-    if (row < end && a.dq)
-      for (int d = lane; d < a.dim; d += 64) ((T*)a.dq)[(row * a.heads + h) * a.dim + d] = (T)0.0f;
-  } else {
-    const PaSeq w = pa_seq(a.s, a.nq, a.nk, span - 1);
-    if (row < w.q0 + w.lq) pa_row_dq<T>(a, w, (int)(row - w.q0), h, hist);
-  }
-  for (int c = 0; c < nb; ++c) {
-    const float s = wave_sum(hist[c * 64 + lane]);
-    if (lane == 0) a.part[(slot * a.heads + h) * nb + c] = s;
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(64 * WAVES) void pa_dkv_rows_kernel(PaArgs a) {
-  const int lane = threadIdx.x & 63;
-  const long item = (long)blockIdx.x * WAVES + (threadIdx.x >> 6);
-  const long slot = item / a.kv_heads;
-  const int g = item % a.kv_heads;
-  if (slot >= (long)a.nk + a.s.batch + 2) return;
-  int start;
-  const int span = pa_span(a.s.cu_k, a.s.batch, a.nk, 0, slot, start);
-  const long row = start + (slot - (long)start - span);
-  int end = span > a.s.batch ? a.nk : pa_clamp(a.s.cu_k[span], a.nk);
-  if (row >= end) return;
-  PaSeq w = {};
-  if (span > 0 && span <= a.s.batch) w = pa_seq(a.s, a.nq, a.nk, span - 1);
-  if (row - start < w.lk) {
-    pa_row_dkv<T>(a, w, (int)(row - start), g);
-    return;
-  }
-  for (int d = lane; d < a.dim; d += 64) {
-    const long at = (row * a.kv_heads + g) * a.dim + d;
-    ((T*)a.dk)[at] = ((T*)a.dv)[at] = (T)0.0f;
-  }
 }
 
 // dtable[h][c] = sum of the parts, in a fixed order: each thread a stride of them, then a tree
@@ -137,8 +87,10 @@ extern "C" int i2r_packed_attention_fwd(const i2r_packed_seqs* seqs, const void*
   return i2r_check_launch("packed_attention_fwd");
 }
 
+static long q_slots(int nq, int batch) { return (nq >> 7) + batch + 2; }
+
 extern "C" long i2r_packed_attention_bwd_ws_bytes(int, int batch, int nq, int, int heads, int, int, int num_buckets) {
-  return ((long)nq * heads + ((long)nq + batch + 2) * heads * num_buckets) * 4;
+  return ((long)nq * heads + q_slots(nq, batch) * heads * num_buckets) * 4;
 }
 
 extern "C" int i2r_packed_attention_bwd(const i2r_packed_seqs* seqs, const void* q, const void* k, const void* v,
@@ -153,6 +105,7 @@ extern "C" int i2r_packed_attention_bwd(const i2r_packed_seqs* seqs, const void*
   I2R_REQUIRE(((uintptr_t)out32 | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0,
               "packed_attention_bwd: tensors have to be 16-byte aligned");
   I2R_REQUIRE(!dk == !dv, "packed_attention_bwd: dk and dv come together");
+  I2R_REQUIRE((long)heads * dim < 1 << 22, "packed_attention_bwd: more than 2^22 elements a row");
   I2R_REQUIRE(table || !dtable, "packed_attention_bwd: dtable without a table");
   const int nb = dtable ? seqs->num_buckets : 0;
   I2R_REQUIRE(ws_bytes >= i2r_packed_attention_bwd_ws_bytes(dtype, seqs->batch, nq, nk, heads, kv_heads, dim, nb) &&
@@ -165,13 +118,11 @@ extern "C" int i2r_packed_attention_bwd(const i2r_packed_seqs* seqs, const void*
   a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)ws, a.part = dtable ? (float*)ws + (long)nq * heads : nullptr;
   a.nq = nq, a.nk = nk, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.scale = scale;
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  const long slots_q = (long)nq + seqs->batch + 2, slots_k = (long)nk + seqs->batch + 2;
-  I2R_REQUIRE(slots_q * heads / WAVES < INT32_MAX && slots_k * kv_heads / WAVES < INT32_MAX,
-              "packed_attention_bwd: too many rows");
-  if (nq) PA_DISPATCH(pa_delta_kernel, i2r_cdiv((long)nq * heads, WAVES), 0);
-  if (dq || dtable) PA_DISPATCH(pa_dq_rows_kernel, i2r_cdiv(slots_q * heads, WAVES), nb * 64 * 4 * WAVES);
+  const bool need_dq = nq && (dq || dtable), need_dkv = nk && dk;
+  if (nq && need_dkv && !need_dq) PA_DISPATCH(pa_delta_kernel, i2r_cdiv((long)nq * heads, WAVES), 0);
+  if (!pa_launch_bwd(dtype, a, st, need_dq, need_dkv)) return I2R_ERR_HIP;
   if (dtable)
-    hipLaunchKernelGGL(pa_dtable_kernel, dim3(heads, nb), dim3(256), 0, st, a.part, dtable, slots_q, heads, nb);
-  if (dk && nk) PA_DISPATCH(pa_dkv_rows_kernel, i2r_cdiv(slots_k * kv_heads, WAVES), 0);
+    hipLaunchKernelGGL(pa_dtable_kernel, dim3(heads, nb), dim3(256), 0, st, a.part, dtable, nq ? q_slots(nq, seqs->batch) : 0,
+                       heads, nb);
   return i2r_check_launch("packed_attention_bwd");
 }

@@ -1,0 +1,380 @@
+// Backward of packed-sequence attention on the matrix cores.
+//
+// Two kernels, both recomputing the scores: dq (a query a column, keys pass by) and dk / dv (a key a column, the queries of
+// all heads of its group pass by).  Seven products where five would do with dq added up atomically -- but no float is ever
+// added in an order that could change, and nothing but the outputs is written.
+#include "packed_tiles.h"
+
+// fp16 holds no probability below 6e-8 and few digits below 6e-5: there p and ds carry 2^12, taken out at the end.
+template <typename T>
+struct Lift {
+  static constexpr float LOG2 = sizeof(T) == 2 && __is_same(T, f16_t) ? 12.0f : 0.0f;
+  static constexpr float DOWN = LOG2 > 0.0f ? 1.0f / 4096.0f : 1.0f;
+};
+
+struct Entry {
+  float bias;  // log2 units
+  int bucket;
+};
+__device__ __forceinline__ void load_entries(Entry* by_distance, const i2r_packed_seqs& s, const float* table, int h) {
+  for (int n = threadIdx.x; n <= 2 * s.max_distance; n += blockDim.x) {
+    const int b = min((int)s.lut[n], s.num_buckets - 1);
+    by_distance[n] = {pa_log2_units(table[(long)h * s.num_buckets + b]), b};
+  }
+}
+
+template <typename T, int DP>
+struct DqShape {
+  static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
+  typedef Tile<T, DP, KEYS> Tl;
+  static constexpr int BUFFER = 2 * Tl::BYTES + 256;  // k, v, positions
+  static constexpr int PER_SIMD = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+  static int lds(bool bias, int max_distance, int hist_buckets) {
+    return 2 * BUFFER + (bias ? (2 * max_distance + 1) * 8 + hist_buckets * 64 * 4 * WAVES : 0);
+  }
+};
+
+// dq of 32 queries a wave, delta = <dout, out> on the way, and ds summed by bucket: each lane its own column of a histogram
+// in LDS, so that no two lanes add to one word.
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, (DqShape<T, DP>::PER_SIMD)) void pa_dq_kernel(PaArgs a, long slots) {
+  typedef DqShape<T, DP> S;
+  typedef typename S::Tl Tl;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  long slot;
+  int h, start;
+  if (!tile_of(slots, a.heads, slot, h)) return;
+  slot = slots - 1 - slot;
+  const bool sums = BIAS && a.part;
+  const int nb = a.s.num_buckets;
+  const int span = pa_span(a.s.cu_q, a.s.batch, a.nq, 7, slot, start);
+  const long row0 = start + ((slot - (start >> 7) - span) << 7);
+  PaSeq w = {};
+  if (span > 0 && span <= a.s.batch) w = pa_seq(a.s, a.nq, a.nk, span - 1);
+  if (row0 >= w.q0 + w.lq) {
+    if (span == 0 || span > a.s.batch) {  // rows of no sequence
+      const int end = (int)min(row0 + S::ROWS, (long)(span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq));
+      if (a.dq)
+        for (long i = (row0 * a.dim) + threadIdx.x; i < (long)end * a.dim; i += 256)
+          ((T*)a.dq)[(i / a.dim * a.heads + h) * a.dim + i % a.dim] = (T)0.0f;
+    }
+    if (sums && threadIdx.x < nb) a.part[(slot * a.heads + h) * nb + threadIdx.x] = 0.0f;
+    return;
+  }
+  const int g = h / (a.heads / a.kv_heads);
+  const int i0 = (int)(row0 - w.q0), iw = i0 + wave * 32, i = iw + col;
+  const bool valid = i < w.lq;
+  const int ahead = w.lk - w.lq;
+  int keys = w.lk;
+  if (a.s.causal) keys = min(keys, min(i0 + S::ROWS, w.lq) + ahead);
+
+  Loader<T, DP, S::KEYS, S::WAVES> lk, lv;
+  lk.init((const T*)a.k + (long)w.k0 * a.k_row + g * a.k_head, a.k_row, a.dim);
+  lv.init((const T*)a.v + (long)w.k0 * a.v_row + g * a.v_head, a.v_row, a.dim);
+  const int far = a.s.max_distance;
+  Entry* by_distance = (Entry*)(lds + 2 * S::BUFFER);
+  float* hist = (float*)(by_distance + 2 * far + 1) + wave * nb * 64;
+  auto load = [&](int n) {
+    char* b = lds + (n & 1) * S::BUFFER;
+    lk.load(b, n * S::KEYS, keys);
+    lv.load(b + Tl::BYTES, n * S::KEYS, keys);
+    if (BIAS && a.s.pos_k) load_words(b + 2 * Tl::BYTES, a.s.pos_k + w.k0, n * S::KEYS, keys);
+  };
+  const int tiles = keys > 0 ? (keys + S::KEYS - 1) / S::KEYS : 0;
+  if (tiles > 0) load(0);
+
+  const long at = ((long)(w.q0 + i) * a.heads + h) * a.dim;
+  frag_t<T> q[Tl::STEPS], dout[Tl::STEPS];
+  load_rows<T>(q, (const T*)a.q + (long)(w.q0 + i) * a.q_row + h * a.q_head, valid, a.dim, half);
+  load_rows<T>(dout, (const T*)a.dout + at, valid, a.dim, half);
+  float delta = 0.0f;
+  if (valid)
+#pragma unroll
+    for (int s = 0; s < Tl::STEPS; ++s) {
+      constexpr int N = 16 / sizeof(T);
+      const int d = (2 * s + half) * N;
+      if (d < a.dim)
+#pragma unroll
+        for (int e = 0; e < N; ++e) delta = fmaf((float)dout[s][e], a.out32_in[at + d + e], delta);
+    }
+  delta += other_half(delta);
+  const long st = (long)h * a.nq + w.q0 + i;
+  const float m = valid ? a.stats[st] : 0.0f, ll = (valid ? a.stats[st + (long)a.heads * a.nq] : INFINITY) - Lift<T>::LOG2;
+  if (valid && half == 0) a.delta[st] = delta;
+  const float sc = a.scale * PA_LOG2E;
+  const int pos_q = BIAS && valid ? pa_pos_q(a.s, w, i) : 0;
+  if (BIAS) load_entries(by_distance, a.s, a.table, h);
+  if (sums)
+    for (int c = 0; c < nb; ++c) hist[c * 64 + lane] = 0.0f;
+
+  f32x16 dq[Tl::BLOCKS];
+#pragma unroll
+  for (int b = 0; b < Tl::BLOCKS; ++b) dq[b] = (f32x16)0.0f;
+
+  for (int n = 0; n < tiles; ++n) {
+    tiles_ready();
+    if (n + 1 < tiles) load(n + 1);
+    const char* kt = lds + (n & 1) * S::BUFFER;
+    const char* vt = kt + Tl::BYTES;
+    const int j0 = n * S::KEYS;
+    if (iw >= w.lq || (a.s.causal && j0 > iw + 31 + ahead)) continue;
+#pragma unroll
+    for (int kb = 0; kb < S::KEYS / 32; ++kb) {
+      const int jb = j0 + kb * 32;
+      f32x16 x = (f32x16)0.0f, dp = (f32x16)0.0f;
+#pragma unroll
+      for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(kt, kb * 32 + col, s, half), q[s]);
+#pragma unroll
+      for (int s = 0; s < Tl::STEPS; ++s) mma_step(dp, Tl::frag(vt, kb * 32 + col, s, half), dout[s]);
+      const int last = a.s.causal ? min(keys, i + ahead + 1) : keys;
+      const bool mask = jb + 32 > keys || (a.s.causal && jb + 31 > iw + ahead);
+      if (BIAS) {
+        const int lo = jb - (iw + 31 + ahead), hi = jb + 31 - (iw + ahead);
+        const bool one = !a.s.pos_q && (hi <= -far || lo >= far);
+        const Entry all = by_distance[hi <= -far ? 0 : 2 * far];
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = acc_row(r, half);
+          Entry e = all;
+          if (!one) {
+            const int pos_k = a.s.pos_k ? ((const int*)(vt + Tl::BYTES))[kb * 32 + row] : jb + row;
+            e = by_distance[pa_entry(pa_apart(pos_k, pos_q), far)];
+          }
+          // hidden by the mask or by its bucket, whatever the key and its value hold
+          const bool open = (!mask || jb + row < last) && e.bias != -INFINITY;
+          const float p = __builtin_amdgcn_exp2f((fmaf(x[r], sc, e.bias) - m) - ll);
+          x[r] = open ? p * (dp[r] - delta) : 0.0f;
+          if (one) sum += x[r];
+          else if (sums)
+            __hip_atomic_fetch_add(hist + e.bucket * 64 + lane, x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        if (one && sums)
+          __hip_atomic_fetch_add(hist + all.bucket * 64 + lane, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      } else {
+        const float ref = m + ll;
+        if (mask) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -ref));
+            x[r] = jb + acc_row(r, half) < last ? p * (dp[r] - delta) : 0.0f;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -ref)) * (dp[r] - delta);
+        }
+      }
+      Probs<T> ds;  // rounded to the type for the product: half a step each, as much as rounding dq once more
+      ds.set(x);
+#pragma unroll
+      for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(kt, kb * 32, b, lane, ds, dq[b]);
+    }
+  }
+
+  float finite = 0.0f;
+  if (a.dq)
+#pragma unroll
+    for (int b = 0; b < Tl::BLOCKS; ++b)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int d = b * 32 + 8 * t + 4 * half;
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float z = dq[b][4 * t + e] * (a.scale * Lift<T>::DOWN);
+          finite = fmaf(z, 0.0f, finite);
+          y[e] = (T)z;
+        }
+        if (valid && d < a.dim) *(t4*)((T*)a.dq + at + d) = y;
+      }
+  if (sums) {
+    __syncthreads();
+    const float* all = (const float*)(by_distance + 2 * far + 1);
+    for (int c = wave; c < nb; c += S::WAVES) {
+      float s = 0.0f;
+      for (int v = 0; v < S::WAVES; ++v) s += all[(v * nb + c) * 64 + lane];
+      s = wave_sum(s);
+      if (lane == 0) a.part[(slot * a.heads + h) * nb + c] = s * Lift<T>::DOWN;
+    }
+  }
+  // a hidden pair's 0 times NaN, or a lifted ds beyond fp16: pair by pair
+  const unsigned long long again = __ballot(valid && !(finite == 0.0f));
+  for (unsigned rows = (unsigned)again | (unsigned)(again >> 32); rows; rows &= rows - 1)
+    pa_row_dq<T>(a, w, iw + __ffs(rows) - 1, h);
+}
+
+template <typename T, int DP>
+struct DkvShape {
+  static constexpr int WAVES = 4, COLS = 32 * WAVES, ROWS = sizeof(T) == 4 ? 32 : 64;
+  typedef Tile<T, DP, ROWS> Tl;
+  static constexpr int BUFFER = 2 * Tl::BYTES + 4 * 256;  // q, dout, two stats, delta, positions
+  static constexpr int PER_SIMD = DP == 128 ? 1 : 2;
+  static int lds(bool bias, int max_distance) { return 2 * BUFFER + (bias ? (2 * max_distance + 1) * 4 : 0); }
+};
+
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kernel(PaArgs a, long slots) {
+  typedef DkvShape<T, DP> S;
+  typedef typename S::Tl Tl;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const int group = a.heads / a.kv_heads;
+  long slot;
+  int g, start;
+  if (!tile_of(slots, a.kv_heads, slot, g)) return;
+  const int span = pa_span(a.s.cu_k, a.s.batch, a.nk, 7, slot, start);
+  const long row0 = start + ((slot - (start >> 7) - span) << 7);
+  const int end = span > a.s.batch ? a.nk : pa_clamp(a.s.cu_k[span], a.nk);  // of the span's rows, keys or not
+  if (row0 >= end) return;
+  PaSeq w = {};
+  if (span > 0 && span <= a.s.batch) w = pa_seq(a.s, a.nq, a.nk, span - 1);
+  const int jg = (int)(row0 - start), jw = jg + wave * 32, j = jw + col;  // first key of workgroup, wave; lane's own
+  const bool valid = j < w.lk;
+  const int ahead = w.lk - w.lq;
+  const int first = a.s.causal ? max(jg - ahead, 0) : 0;  // first query that sees one of the workgroup's keys
+  const int tiles = jg < w.lk && first < w.lq ? (w.lq - first + S::ROWS - 1) / S::ROWS : 0;
+  const int far = a.s.max_distance;
+  float* by_distance = (float*)(lds + 2 * S::BUFFER);
+
+  frag_t<T> k[Tl::STEPS], v[Tl::STEPS];
+  load_rows<T>(k, (const T*)a.k + (long)(w.k0 + j) * a.k_row + g * a.k_head, valid, a.dim, half);
+  load_rows<T>(v, (const T*)a.v + (long)(w.k0 + j) * a.v_row + g * a.v_head, valid, a.dim, half);
+  const float sc = a.scale * PA_LOG2E;
+  const int pos_k = BIAS && valid ? pa_pos_k(a.s, w, j) : 0;
+
+  f32x16 dk[Tl::BLOCKS], dv[Tl::BLOCKS];
+#pragma unroll
+  for (int b = 0; b < Tl::BLOCKS; ++b) dk[b] = dv[b] = (f32x16)0.0f;
+
+  for (int h = g * group; h < (g + 1) * group && tiles > 0; ++h) {
+    Loader<T, DP, S::ROWS, S::WAVES> lq, ld;
+    lq.init((const T*)a.q + (long)w.q0 * a.q_row + h * a.q_head, a.q_row, a.dim);
+    ld.init((const T*)a.dout + ((long)w.q0 * a.heads + h) * a.dim, (long)a.heads * a.dim, a.dim);
+    const float* stats = a.stats + (long)h * a.nq + w.q0;
+    const float* delta = a.delta + (long)h * a.nq + w.q0;
+    auto load = [&](int n) {
+      char* b = lds + (n & 1) * S::BUFFER;
+      const int r = first + n * S::ROWS;
+      lq.load(b, r, w.lq);
+      ld.load(b + Tl::BYTES, r, w.lq);
+      char* e = b + 2 * Tl::BYTES;
+      load_words(e, stats, r, w.lq);
+      load_words(e + 256, stats + (long)a.heads * a.nq, r, w.lq);
+      load_words(e + 512, delta, r, w.lq);
+      if (BIAS && a.s.pos_q) load_words(e + 768, a.s.pos_q + w.q0, r, w.lq);
+    };
+    __syncthreads();  // the last head's tiles and table are read
+    load(0);
+    if (BIAS) load_table(by_distance, a.s, a.table, h);
+    for (int n = 0; n < tiles; ++n) {
+      tiles_ready();
+      if (n + 1 < tiles) load(n + 1);
+      const char* qt = lds + (n & 1) * S::BUFFER;
+      const char* dt = qt + Tl::BYTES;
+      const float* rows = (const float*)(dt + Tl::BYTES);
+      const int i0 = first + n * S::ROWS;
+      if (jw >= w.lk || (a.s.causal && jw > i0 + S::ROWS - 1 + ahead)) continue;
+#pragma unroll
+      for (int qb = 0; qb < S::ROWS / 32; ++qb) {
+        const int ib = i0 + qb * 32;
+        f32x16 x = (f32x16)0.0f, dp = (f32x16)0.0f;
+#pragma unroll
+        for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(qt, qb * 32 + col, s, half), k[s]);
+#pragma unroll
+        for (int s = 0; s < Tl::STEPS; ++s) mma_step(dp, Tl::frag(dt, qb * 32 + col, s, half), v[s]);
+        const bool mask = ib + 32 > w.lq || (a.s.causal && jw + 31 > ib + ahead);
+        const int lo = jw - (ib + 31 + ahead), hi = jw + 31 - (ib + ahead);
+        const bool one = BIAS && !a.s.pos_q && (hi <= -far || lo >= far);
+        const float all = BIAS ? by_distance[hi <= -far ? 0 : 2 * far] : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = qb * 32 + acc_row(r, half), i = i0 + row;
+          const float m = rows[row], ll = rows[64 + row] - Lift<T>::LOG2;
+          float p;
+          bool open = !mask || (i < w.lq && (!a.s.causal || j <= i + ahead));
+          if (BIAS) {
+            float e = all;
+            if (!one) {
+              const int pos_q = a.s.pos_q ? ((const int*)rows)[192 + row] : i + ahead;
+              e = by_distance[pa_entry(pa_apart(pos_k, pos_q), far)];
+            }
+            open = open && e != -INFINITY;
+            p = __builtin_amdgcn_exp2f((fmaf(x[r], sc, e) - m) - ll);
+          } else {
+            p = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -(m + ll)));
+          }
+          x[r] = open ? p : 0.0f;
+          dp[r] = open ? p * (dp[r] - rows[128 + row]) : 0.0f;
+        }
+        Probs<T> pp, ds;  // rounded to the type: half a step each
+        pp.set(x);
+        ds.set(dp);
+#pragma unroll
+        for (int b = 0; b < Tl::BLOCKS; ++b) {
+          Tl::mma_t(dt, qb * 32, b, lane, pp, dv[b]);
+          Tl::mma_t(qt, qb * 32, b, lane, ds, dk[b]);
+        }
+      }
+    }
+  }
+
+  float finite = 0.0f;
+  const bool there = row0 + wave * 32 + col < end;  // keys' gradients, and zeros behind a sequence's keys
+  const long at = ((row0 + wave * 32 + col) * a.kv_heads + g) * a.dim;
+#pragma unroll
+  for (int b = 0; b < Tl::BLOCKS; ++b)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int d = b * 32 + 8 * t + 4 * half;
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      t4 y, z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float fk = dk[b][4 * t + e] * (a.scale * Lift<T>::DOWN), fv = dv[b][4 * t + e] * Lift<T>::DOWN;
+        finite = fmaf(fk, 0.0f, fmaf(fv, 0.0f, finite));
+        y[e] = valid ? (T)fk : (T)0.0f;
+        z[e] = valid ? (T)fv : (T)0.0f;
+      }
+      if (there && d < a.dim) *(t4*)((T*)a.dk + at + d) = y, *(t4*)((T*)a.dv + at + d) = z;
+    }
+  const unsigned long long again = __ballot(valid && !(finite == 0.0f));
+  for (unsigned rows = (unsigned)again | (unsigned)(again >> 32); rows; rows &= rows - 1)
+    pa_row_dkv<T>(a, w, jw + __ffs(rows) - 1, g);
+}
+
+#define PA_LAUNCH(KERNEL, SLOTS, HEADS, LDS, MOST)                                                         \
+  {                                                                                                        \
+    static bool done[64];                                                                                  \
+    if (!i2r_lds_attr((const void*)KERNEL, MOST, done)) return false;                                      \
+    hipLaunchKernelGGL(KERNEL, dim3(tile_grid(SLOTS, HEADS)), dim3(256), LDS, st, a, SLOTS);               \
+  }
+
+template <typename T, int DP>
+static bool launch_bwd(const PaArgs& a, hipStream_t st, bool dq, bool dkv) {
+  const int far = a.s.max_distance;
+  const long slots_q = (a.nq >> 7) + a.s.batch + 2, slots_k = (a.nk >> 7) + a.s.batch + 2;
+  if (dq) {
+    typedef DqShape<T, DP> S;
+    if (a.table) PA_LAUNCH((pa_dq_kernel<T, DP, true>), slots_q, a.heads, S::lds(true, far, a.part ? a.s.num_buckets : 0),
+                           S::lds(true, PA_MAX_DISTANCE, PA_MAX_BUCKETS))
+    else PA_LAUNCH((pa_dq_kernel<T, DP, false>), slots_q, a.heads, S::lds(false, 0, 0), S::lds(false, 0, 0))
+  }
+  if (dkv) {
+    typedef DkvShape<T, DP> S;
+    if (a.table) PA_LAUNCH((pa_dkv_kernel<T, DP, true>), slots_k, a.kv_heads, S::lds(true, far), S::lds(true, PA_MAX_DISTANCE))
+    else PA_LAUNCH((pa_dkv_kernel<T, DP, false>), slots_k, a.kv_heads, S::lds(false, 0), S::lds(false, 0))
+  }
+  return true;
+}
+
+bool pa_launch_bwd(int dtype, const PaArgs& a, hipStream_t st, bool dq, bool dkv) {
+#define PA_BY_DIM(T)                                            \
+  return a.dim <= 32   ? launch_bwd<T, 32>(a, st, dq, dkv)      \
+         : a.dim <= 64 ? launch_bwd<T, 64>(a, st, dq, dkv)      \
+                       : launch_bwd<T, 128>(a, st, dq, dkv);
+  if (dtype == 0) PA_BY_DIM(float)
+  if (dtype == 1) PA_BY_DIM(f16_t)
+  PA_BY_DIM(bf16_t)
+}

@@ -7,19 +7,9 @@ template <typename T, int DP>
 struct FwdShape {
   static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
   typedef Tile<T, DP, KEYS> Tl;
-  static constexpr int BUFFER = 2 * Tl::BYTES + KEYS * 4;  // k, v, positions
+  static constexpr int BUFFER = 2 * Tl::BYTES + 256;  // k, v, positions
   static int lds(bool bias, int max_distance) { return 2 * BUFFER + (bias ? (2 * max_distance + 1) * 4 : 0); }
 };
-
-// order of the tiles: each of the 8 XCDs (workgroups go to them in turn) works through whole heads, so that a head's keys
-// and values stay in that XCD's L2; within a head the last -- with a causal mask longest -- tiles first
-__device__ __forceinline__ bool tile_of(long slots, int heads, long& slot, int& h) {
-  const long per = (slots * heads + 7) / 8, w = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (w >= slots * heads || (long)(blockIdx.x >> 3) >= per) return false;
-  h = (int)(w / slots);
-  slot = slots - 1 - w % slots;
-  return true;
-}
 
 template <typename T, int DP, bool BIAS, bool SAVE>
 __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
@@ -30,6 +20,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
   long slot;
   int h, start;
   if (!tile_of(slots, a.heads, slot, h)) return;
+  slot = slots - 1 - slot;  // the last tiles of a sequence -- with a causal mask the longest -- first
   const int span = pa_span(a.s.cu_q, a.s.batch, a.nq, 7, slot, start);
   const long row0 = start + ((slot - (start >> 7) - span) << 7);
   if (span == 0 || span > a.s.batch) {  // rows of no sequence
@@ -59,10 +50,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
     char* b = lds + (n & 1) * S::BUFFER;
     lk.load(b, n * S::KEYS, keys);
     lv.load(b + Tl::BYTES, n * S::KEYS, keys);
-    if (BIAS && a.s.pos_k && threadIdx.x < S::KEYS) {
-      const int j = n * S::KEYS + threadIdx.x;
-      ((int*)(b + 2 * Tl::BYTES))[threadIdx.x] = j < keys ? a.s.pos_k[w.k0 + j] : 0;
-    }
+    if (BIAS && a.s.pos_k) load_words(b + 2 * Tl::BYTES, a.s.pos_k + w.k0, n * S::KEYS, keys);
   };
   const int tiles = keys > 0 ? (keys + S::KEYS - 1) / S::KEYS : 0;
   if (tiles > 0) load(0);
@@ -193,7 +181,7 @@ static void launch_fwd(const PaArgs& a, hipStream_t st, bool& ok) {
   const bool bias = a.table != nullptr, save = a.stats != nullptr;
   const long slots = (a.nq >> 7) + a.s.batch + 2;
   const int lds = S::lds(bias, a.s.max_distance);
-  const dim3 grid((unsigned)((slots * a.heads + 7) / 8 * 8));
+  const dim3 grid(tile_grid(slots, a.heads));
 #define PA_FWD(B, V)                                                                                \
   {                                                                                                 \
     static bool done[64];                                                                           \

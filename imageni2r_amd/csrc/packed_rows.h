@@ -76,8 +76,9 @@ __device__ __forceinline__ float pa_score(const PaArgs& a, const PaSeq& w, int h
   float b = 0.0f;
   bucket = 0;
   if (a.table) {
-    bucket = a.s.lut[pa_entry(pa_apart(pa_pos_k(a.s, w, j), pos_q), a.s.max_distance)];
+    bucket = min((int)a.s.lut[pa_entry(pa_apart(pa_pos_k(a.s, w, j), pos_q), a.s.max_distance)], a.s.num_buckets - 1);
     b = pa_log2_units(a.table[(long)h * a.s.num_buckets + bucket]);
+    if (b == -INFINITY) return b;  // hidden, whatever the key holds
   }
   return fmaf(pa_dot(qi, kj, a.dim), a.scale * PA_LOG2E, b);
 }
@@ -140,9 +141,9 @@ __device__ __forceinline__ void pa_pair(const PaArgs& a, float x, long row, int 
   ds = p * (pa_dot(doi, vj, a.dim) - a.delta[at]);
 }
 
-// dq of query i, head h; `hist` (num_buckets x 64 floats of this wave's own): ds added by bucket, a column for each lane.
+// dq of query i, head h.
 template <typename T>
-__device__ __forceinline__ void pa_row_dq(const PaArgs& a, const PaSeq& w, int i, int h, float* hist) {
+__device__ __forceinline__ void pa_row_dq(const PaArgs& a, const PaSeq& w, int i, int h) {
   const int lane = threadIdx.x & 63, g = h / (a.heads / a.kv_heads);
   const long row = w.q0 + i, at = (row * a.heads + h) * a.dim;
   const T* qi = (const T*)a.q + row * a.q_row + h * a.q_head;
@@ -156,10 +157,7 @@ __device__ __forceinline__ void pa_row_dq(const PaArgs& a, const PaSeq& w, int i
     float x = -INFINITY, p = 0.0f, ds = 0.0f;
     if (j < seen) {
       x = pa_score(a, w, h, qi, (const T*)a.k + (long)(w.k0 + j) * a.k_row + g * a.k_head, pos_q, j, bucket);
-      if (!(x == -INFINITY)) {
-        pa_pair(a, x, row, h, doi, (const T*)a.v + (long)(w.k0 + j) * a.v_row + g * a.v_head, p, ds);
-        if (hist) hist[bucket * 64 + lane] += ds;
-      }
+      if (!(x == -INFINITY)) pa_pair(a, x, row, h, doi, (const T*)a.v + (long)(w.k0 + j) * a.v_row + g * a.v_head, p, ds);
     }
     for (unsigned long long open = __ballot(!(x == -INFINITY)); open; open &= open - 1) {
       const int t = __ffsll(open) - 1;

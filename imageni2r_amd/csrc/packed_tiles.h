@@ -173,7 +173,35 @@ __device__ __forceinline__ void tiles_ready() {
   asm volatile("" ::: "memory");
 }
 
-// The table of one head by distance, in log2 units, and the bucket numbers beside it.
+// 4 bytes for each of up to 64 rows into LDS, by wave 0 (in flight until the next tiles_ready()); rows behind the last: 0
+__device__ __forceinline__ void load_words(void* to, const void* from, int first, int rows) {
+  if (threadIdx.x >= 64) return;
+  const int left = min(rows - first, 64);
+  const unsigned long long at = (unsigned long long)((const int*)from + first);
+  i32x4 rs;
+  rs[0] = __builtin_amdgcn_readfirstlane((int)at);
+  rs[1] = __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff);
+  rs[2] = __builtin_amdgcn_readfirstlane(max(left, 0) * 4);
+  rs[3] = 0x00020000;
+  const int lds = __builtin_amdgcn_readfirstlane((int)(unsigned long)LDS_PTR(char, to));
+  asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"((int)threadIdx.x * 4), "s"(rs)
+               : "memory");
+}
+
+// Order of the tiles: each of the 8 XCDs (workgroups go to them in turn) works through whole heads, so that what a head's
+// workgroups all read stays in that XCD's L2.
+__device__ __forceinline__ bool tile_of(long slots, int heads, long& slot, int& h) {
+  const long per = (slots * heads + 7) / 8, w = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (w >= slots * heads || (long)(blockIdx.x >> 3) >= per) return false;
+  h = (int)(w / slots);
+  slot = w % slots;
+  return true;
+}
+static inline unsigned tile_grid(long slots, int heads) { return (unsigned)((slots * heads + 7) / 8 * 8); }
+
+// One head's bias by distance, in log2 units.
 __device__ __forceinline__ void load_table(float* by_distance, const i2r_packed_seqs& s, const float* table, int h) {
   for (int n = threadIdx.x; n <= 2 * s.max_distance; n += blockDim.x)
     by_distance[n] = pa_log2_units(table[(long)h * s.num_buckets + min((int)s.lut[n], s.num_buckets - 1)]);
