@@ -2,6 +2,9 @@
 #include "packed_rows.h"
 
 bool pa_launch_fwd(int dtype, const PaArgs& a, hipStream_t st);  // packed_fwd.hip
+bool pa_is_token(int batch, int nq, int heads, int kv_heads);  // packed_token.hip
+long pa_token_ws_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim);
+bool pa_launch_token(int dtype, const PaArgs& a, void* ws, hipStream_t st);
 bool pa_launch_bwd(int dtype, const PaArgs& a, hipStream_t st, bool dq, bool dkv);  // packed_bwd.hip
 
 #define WAVES 4  // rows a workgroup works on, one wave each
@@ -42,6 +45,7 @@ static int check(const char* what, const i2r_packed_seqs* s, const void* q, cons
   I2R_REQUIRE(nq >= 0 && nk >= 0 && nq < 1 << 30 && nk < 1 << 30, "%s: 0 to 2^30 - 1 rows are supported", what);
   I2R_REQUIRE(kv_heads > 0 && heads > 0 && heads < 65536 && heads % kv_heads == 0, "%s: %d heads are no multiple of %d key / value heads",
               what, heads, kv_heads);
+  I2R_REQUIRE(((long)std::max(nq, nk) + s->batch + 2) * heads < INT32_MAX / 2, "%s: too many rows times heads", what);
   I2R_REQUIRE(dim >= 8 && dim <= 128 && dim % 8 == 0, "%s: head dim %d is not a multiple of 8 up to 128", what, dim);
   I2R_REQUIRE((q || !nq) && (k || !nk) && (v || !nk), "%s: null tensor", what);
   I2R_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: q, k and v have to be 16-byte aligned", what);
@@ -65,7 +69,10 @@ static int check(const char* what, const i2r_packed_seqs* s, const void* q, cons
     default: hipLaunchKernelGGL(KERNEL<bf16_t>, dim3(GRID), dim3(64 * WAVES), LDS, st, a); break;     \
   }
 
-extern "C" long i2r_packed_attention_fwd_ws_bytes(int, int, int, int, int, int, int) { return 0; }
+extern "C" long i2r_packed_attention_fwd_ws_bytes(int, int batch, int nq, int nk, int heads, int kv_heads, int dim) {
+  if (batch <= 0 || nq <= 0 || nk < 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
+  return pa_is_token(batch, nq, heads, kv_heads) ? pa_token_ws_bytes(batch, nq, nk, heads, kv_heads, dim) : 0;
+}
 
 extern "C" int i2r_packed_attention_fwd(const i2r_packed_seqs* seqs, const void* q, const void* k, const void* v,
                                         const float* table, void* out, float* out32, float* stats, void* ws, long ws_bytes,
@@ -83,7 +90,12 @@ extern "C" int i2r_packed_attention_fwd(const i2r_packed_seqs* seqs, const void*
   a.q = q, a.k = k, a.v = v, a.table = table, a.out = out, a.out32 = out32, a.stats = stats;
   a.nq = nq, a.nk = nk, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.scale = scale, a.zero_outside = zero_outside;
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  if (!pa_launch_fwd(dtype, a, st)) return I2R_ERR_HIP;
+  const long need = i2r_packed_attention_fwd_ws_bytes(dtype, seqs->batch, nq, nk, heads, kv_heads, dim);
+  I2R_REQUIRE(ws_bytes >= need && (ws || !need), "packed_attention_fwd: workspace of %ld bytes, %ld are needed", ws_bytes,
+              need);
+  I2R_REQUIRE((uintptr_t)ws % 16 == 0, "packed_attention_fwd: the workspace has to be 16-byte aligned");
+  if (!(pa_is_token(seqs->batch, nq, heads, kv_heads) ? pa_launch_token(dtype, a, ws, st) : pa_launch_fwd(dtype, a, st)))
+    return I2R_ERR_HIP;
   return i2r_check_launch("packed_attention_fwd");
 }
 

@@ -105,7 +105,8 @@ struct Probs<float> {
   __device__ __forceinline__ void set(const f32x16& x) { f = x; }
 };
 
-// Loads tiles of rows of one (sequence, head) into LDS without passing through registers.  Rows behind the last and
+// Loads tiles of rows of one (sequence, head) into LDS without passing through registers, by WAVES waves together or (1)
+// by each wave for itself.  Rows behind the last and
 // columns behind the head dim are out of the descriptor's range and arrive as zeros.
 template <typename T, int DP, int ROWS, int WAVES>
 struct Loader {
@@ -119,7 +120,7 @@ struct Loader {
 
   __device__ __forceinline__ void init(const T* p, long row_stride, int dim) {
     base = (const char*)p, step = row_stride * (long)sizeof(T), width = dim * (int)sizeof(T);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int chunk = (i * WAVES + wave) * 64 + lane, row = chunk / Tl::CHUNKS;
@@ -137,7 +138,7 @@ struct Loader {
     rs[1] = __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff);
     rs[2] = __builtin_amdgcn_readfirstlane(left > 0 ? (int)((left - 1) * step) + width : 0);
     rs[3] = 0x00020000;
-    const int to = __builtin_amdgcn_readfirstlane((int)(unsigned long)LDS_PTR(char, tile) + (threadIdx.x >> 6) * 1024);
+    const int to = __builtin_amdgcn_readfirstlane((int)(unsigned long)LDS_PTR(char, tile) + (WAVES == 1 ? 0 : (threadIdx.x >> 6) * 1024));
     asm volatile("s_nop 4" : : "s"(rs), "s"(to));  // a vector instruction may have written them just before
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
