@@ -7,19 +7,20 @@ long pa_token_ws_bytes(int batch, int nq, int nk, int heads, int kv_heads, int d
 bool pa_launch_token(int dtype, const PaArgs& a, void* ws, hipStream_t st);
 bool pa_launch_bwd(int dtype, const PaArgs& a, hipStream_t st, bool dq, bool dkv);  // packed_bwd.hip
 
-#define WAVES 4  // rows a workgroup works on, one wave each
-
-// delta = <dout, out> of each row and head
+// delta = <dout, out> of each row and head, and the sum of its stats: for dk and dv without dq.  Two threads for each, in the
+// dq kernel's order, so that the gradients do not depend on which of them are asked for.
 template <typename T>
-__global__ __launch_bounds__(64 * WAVES) void pa_delta_kernel(PaArgs a) {
-  const int lane = threadIdx.x & 63;
-  const long item = (long)blockIdx.x * WAVES + (threadIdx.x >> 6);
-  if (item >= (long)a.nq * a.heads) return;
+__global__ __launch_bounds__(256) void pa_delta_kernel(PaArgs a) {
+  constexpr int N = 16 / sizeof(T);
+  const long item = (long)blockIdx.x * 128 + (threadIdx.x >> 1);
   const long row = item / a.heads, at = item * a.dim;
   float s = 0.0f;
-  for (int d = lane; d < a.dim; d += 64) s = fmaf((float)((const T*)a.dout)[at + d], a.out32_in[at + d], s);
-  s = wave_sum(s);
-  if (lane == 0) a.delta[(item % a.heads) * a.nq + row] = s;
+  if (row < a.nq)
+    for (int d = (threadIdx.x & 1) * N; d < a.dim; d += 2 * N)
+      for (int e = 0; e < N; ++e) s = fmaf((float)((const T*)a.dout)[at + d + e], a.out32_in[at + d + e], s);
+  s += __shfl_xor(s, 1, 64);
+  const long st = (item % a.heads) * a.nq + row, n = (long)a.heads * a.nq;
+  if (row < a.nq && !(threadIdx.x & 1)) a.delta[st] = s, a.delta[st + n] = a.stats[st] + (a.stats[st + n] - Lift<T>::LOG2);
 }
 
 // dtable[h][c] = sum of the parts, in a fixed order: each thread a stride of them, then a tree
@@ -62,13 +63,6 @@ static int check(const char* what, const i2r_packed_seqs* s, const void* q, cons
   return I2R_OK;
 }
 
-#define PA_DISPATCH(KERNEL, GRID, LDS)                                                               \
-  switch (dtype) {                                                                                   \
-    case 0: hipLaunchKernelGGL(KERNEL<float>, dim3(GRID), dim3(64 * WAVES), LDS, st, a); break;       \
-    case 1: hipLaunchKernelGGL(KERNEL<f16_t>, dim3(GRID), dim3(64 * WAVES), LDS, st, a); break;       \
-    default: hipLaunchKernelGGL(KERNEL<bf16_t>, dim3(GRID), dim3(64 * WAVES), LDS, st, a); break;     \
-  }
-
 extern "C" long i2r_packed_attention_fwd_ws_bytes(int, int batch, int nq, int nk, int heads, int kv_heads, int dim) {
   if (batch <= 0 || nq <= 0 || nk < 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
   return pa_is_token(batch, nq, heads, kv_heads) ? pa_token_ws_bytes(batch, nq, nk, heads, kv_heads, dim) : 0;
@@ -102,7 +96,7 @@ extern "C" int i2r_packed_attention_fwd(const i2r_packed_seqs* seqs, const void*
 static long q_slots(int nq, int batch) { return (nq >> 7) + batch + 2; }
 
 extern "C" long i2r_packed_attention_bwd_ws_bytes(int, int batch, int nq, int, int heads, int, int, int num_buckets) {
-  return ((long)nq * heads + q_slots(nq, batch) * heads * num_buckets) * 4;
+  return (2 * (long)nq * heads + q_slots(nq, batch) * heads * num_buckets) * 4;
 }
 
 extern "C" int i2r_packed_attention_bwd(const i2r_packed_seqs* seqs, const void* q, const void* k, const void* v,
@@ -127,11 +121,16 @@ extern "C" int i2r_packed_attention_bwd(const i2r_packed_seqs* seqs, const void*
   PaArgs a = {};
   a.s = *seqs;
   a.q = q, a.k = k, a.v = v, a.table = table, a.out32_in = out32, a.stats = (float*)stats, a.dout = dout;
-  a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)ws, a.part = dtable ? (float*)ws + (long)nq * heads : nullptr;
+  a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)ws, a.part = dtable ? (float*)ws + 2 * (long)nq * heads : nullptr;
   a.nq = nq, a.nk = nk, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.scale = scale;
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
   const bool need_dq = nq && (dq || dtable), need_dkv = nk && dk;
-  if (nq && need_dkv && !need_dq) PA_DISPATCH(pa_delta_kernel, i2r_cdiv((long)nq * heads, WAVES), 0);
+  if (nq && need_dkv && !need_dq) {
+    const dim3 grid(i2r_cdiv((long)nq * heads, 128));
+    if (dtype == 0) hipLaunchKernelGGL(pa_delta_kernel<float>, grid, dim3(256), 0, st, a);
+    else if (dtype == 1) hipLaunchKernelGGL(pa_delta_kernel<f16_t>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(pa_delta_kernel<bf16_t>, grid, dim3(256), 0, st, a);
+  }
   if (!pa_launch_bwd(dtype, a, st, need_dq, need_dkv)) return I2R_ERR_HIP;
   if (dtable)
     hipLaunchKernelGGL(pa_dtable_kernel, dim3(heads, nb), dim3(256), 0, st, a.part, dtable, nq ? q_slots(nq, seqs->batch) : 0,

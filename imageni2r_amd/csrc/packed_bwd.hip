@@ -5,13 +5,6 @@
 // added in an order that could change, and nothing but the outputs is written.
 #include "packed_tiles.h"
 
-// fp16 holds no probability below 6e-8 and few digits below 6e-5: there p and ds carry 2^12, taken out at the end.
-template <typename T>
-struct Lift {
-  static constexpr float LOG2 = sizeof(T) == 2 && __is_same(T, f16_t) ? 12.0f : 0.0f;
-  static constexpr float DOWN = LOG2 > 0.0f ? 1.0f / 4096.0f : 1.0f;
-};
-
 struct Entry {
   float bias;  // log2 units
   int bucket;
@@ -28,20 +21,22 @@ struct DqShape {
   static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
   typedef Tile<T, DP, KEYS> Tl;
   static constexpr int BUFFER = 2 * Tl::BYTES + 256;  // k, v, positions
-  static constexpr int PER_SIMD = sizeof(T) == 4 && DP == 128 ? 1 : 2;
-  static int lds(bool bias, int max_distance, int hist_buckets) {
-    return 2 * BUFFER + (bias ? (2 * max_distance + 1) * 8 + hist_buckets * 64 * 4 * WAVES : 0);
+  static constexpr int PER_SIMD = sizeof(T) == 4 && DP == 128 ? 1 : 2, UNROLL = DP == 128 ? 1 : 2;
+  static constexpr bool APART = DP == 128;  // the products' operands would not fit the registers all at once
+  static int lds(bool bias, int max_distance, int buckets) {
+    return 2 * BUFFER + (bias ? (2 * max_distance + 1) * 8 + buckets * 64 * 4 * WAVES : 0);
   }
 };
 
-// dq of 32 queries a wave, delta = <dout, out> on the way, and ds summed by bucket: each lane its own column of a histogram
+// dq of 32 queries a wave, delta = <dout, out> and the two stats' sum on the way for the other kernel, and ds summed by bucket: each lane its own column of a histogram
 // in LDS, so that no two lanes add to one word.
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, (DqShape<T, DP>::PER_SIMD)) void pa_dq_kernel(PaArgs a, long slots) {
   typedef DqShape<T, DP> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31,
+            half = lane >> 5;
   long slot;
   int h, start;
   if (!tile_of(slots, a.heads, slot, h)) return;
@@ -84,10 +79,10 @@ __global__ __launch_bounds__(256, (DqShape<T, DP>::PER_SIMD)) void pa_dq_kernel(
   const int tiles = keys > 0 ? (keys + S::KEYS - 1) / S::KEYS : 0;
   if (tiles > 0) load(0);
 
-  const long at = ((long)(w.q0 + i) * a.heads + h) * a.dim;
+  const long to = ((long)(w.q0 + i) * a.heads + h) * a.dim;
   frag_t<T> q[Tl::STEPS], dout[Tl::STEPS];
   load_rows<T>(q, (const T*)a.q + (long)(w.q0 + i) * a.q_row + h * a.q_head, valid, a.dim, half);
-  load_rows<T>(dout, (const T*)a.dout + at, valid, a.dim, half);
+  load_rows<T>(dout, (const T*)a.dout + to, valid, a.dim, half);
   float delta = 0.0f;
   if (valid)
 #pragma unroll
@@ -96,80 +91,104 @@ __global__ __launch_bounds__(256, (DqShape<T, DP>::PER_SIMD)) void pa_dq_kernel(
       const int d = (2 * s + half) * N;
       if (d < a.dim)
 #pragma unroll
-        for (int e = 0; e < N; ++e) delta = fmaf((float)dout[s][e], a.out32_in[at + d + e], delta);
+        for (int e = 0; e < N; ++e) delta = fmaf((float)dout[s][e], a.out32_in[to + d + e], delta);
     }
   delta += other_half(delta);
   const long st = (long)h * a.nq + w.q0 + i;
   const float m = valid ? a.stats[st] : 0.0f, ll = (valid ? a.stats[st + (long)a.heads * a.nq] : INFINITY) - Lift<T>::LOG2;
-  if (valid && half == 0) a.delta[st] = delta;
+  const float ref = m + ll;
+  if (valid && half == 0) a.delta[st] = delta, a.delta[st + (long)a.heads * a.nq] = ref;
   const float sc = a.scale * PA_LOG2E;
   const int pos_q = BIAS && valid ? pa_pos_q(a.s, w, i) : 0;
   if (BIAS) load_entries(by_distance, a.s, a.table, h);
-  if (sums)
+  if (BIAS)
     for (int c = 0; c < nb; ++c) hist[c * 64 + lane] = 0.0f;
 
   f32x16 dq[Tl::BLOCKS];
 #pragma unroll
   for (int b = 0; b < Tl::BLOCKS; ++b) dq[b] = (f32x16)0.0f;
 
-  for (int n = 0; n < tiles; ++n) {
-    tiles_ready();
-    if (n + 1 < tiles) load(n + 1);
-    const char* kt = lds + (n & 1) * S::BUFFER;
+  typename Tl::Lane at(lane);
+  auto tile = [&](auto masked, auto mode, const char* kt, int j0) {
+    constexpr bool MASK = decltype(masked)::value;
+    constexpr int MODE = decltype(mode)::value;
     const char* vt = kt + Tl::BYTES;
-    const int j0 = n * S::KEYS;
-    if (iw >= w.lq || (a.s.causal && j0 > iw + 31 + ahead)) continue;
-#pragma unroll
+    at.fresh();
+    const int last = a.s.causal ? min(keys, i + ahead + 1) : keys;
+#pragma unroll S::UNROLL
     for (int kb = 0; kb < S::KEYS / 32; ++kb) {
-      const int jb = j0 + kb * 32;
       f32x16 x = (f32x16)0.0f, dp = (f32x16)0.0f;
 #pragma unroll
-      for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(kt, kb * 32 + col, s, half), q[s]);
+      for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(kt, kb * 32, s, at), q[s]);
+      if (S::APART) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < Tl::STEPS; ++s) mma_step(dp, Tl::frag(vt, kb * 32 + col, s, half), dout[s]);
-      const int last = a.s.causal ? min(keys, i + ahead + 1) : keys;
-      const bool mask = jb + 32 > keys || (a.s.causal && jb + 31 > iw + ahead);
-      if (BIAS) {
-        const int lo = jb - (iw + 31 + ahead), hi = jb + 31 - (iw + ahead);
-        const bool one = !a.s.pos_q && (hi <= -far || lo >= far);
-        const Entry all = by_distance[hi <= -far ? 0 : 2 * far];
+      for (int s = 0; s < Tl::STEPS; ++s) mma_step(dp, Tl::frag(vt, kb * 32, s, at), dout[s]);
+      if (S::APART) __builtin_amdgcn_sched_barrier(0);
+      if constexpr (MODE == NONE) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float ds = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -ref)) * (dp[r] - delta);
+          x[r] = MASK && !(j0 + kb * 32 + acc_row(r, half) < last) ? 0.0f : ds;
+        }
+      } else {
+        Entry e[16];
+        e[0] = by_distance[j0 < iw + ahead ? 0 : 2 * far];
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int row = acc_row(r, half);
-          Entry e = all;
-          if (!one) {
-            const int pos_k = a.s.pos_k ? ((const int*)(vt + Tl::BYTES))[kb * 32 + row] : jb + row;
-            e = by_distance[pa_entry(pa_apart(pos_k, pos_q), far)];
-          }
-          // hidden by the mask or by its bucket, whatever the key and its value hold
-          const bool open = (!mask || jb + row < last) && e.bias != -INFINITY;
-          const float p = __builtin_amdgcn_exp2f((fmaf(x[r], sc, e.bias) - m) - ll);
-          x[r] = open ? p * (dp[r] - delta) : 0.0f;
-          if (one) sum += x[r];
-          else if (sums)
-            __hip_atomic_fetch_add(hist + e.bucket * 64 + lane, x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          const int row = kb * 32 + acc_row(r, half);
+          if (MODE == ONE) e[r] = e[0];
+          if (MODE == NEAR) e[r] = by_distance[pa_entry(j0 + row - pos_q, far)];
+          if (MODE == GIVEN) e[r] = by_distance[pa_entry(pa_apart(((const int*)(vt + Tl::BYTES))[row], pos_q), far)];
         }
-        if (one && sums)
-          __hip_atomic_fetch_add(hist + all.bucket * 64 + lane, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-      } else {
-        const float ref = m + ll;
-        if (mask) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -ref));
-            x[r] = jb + acc_row(r, half) < last ? p * (dp[r] - delta) : 0.0f;
-          }
+        for (int r = 0; r < 16; ++r) {
+          // hidden by its place or by its bucket: whatever the key and its value hold
+          const bool open = (int)(!MASK || j0 + kb * 32 + acc_row(r, half) < last) & (int)(e[r].bias != -INFINITY);
+          const float p = __builtin_amdgcn_exp2f((fmaf(x[r], sc, e[r].bias) - m) - ll);
+          x[r] = open ? p * (dp[r] - delta) : 0.0f;
+          sum += x[r];
+        }
+        // (after all reads of LDS: an addition may be to any word, for all the compiler knows)
+        if (MODE == ONE) {
+          __hip_atomic_fetch_add(hist + e[0].bucket * 64 + lane, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -ref)) * (dp[r] - delta);
+          for (int r = 0; r < 16; ++r)
+            __hip_atomic_fetch_add(hist + e[r].bucket * 64 + lane, x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
       }
+      if (S::APART) __builtin_amdgcn_sched_barrier(0);
       Probs<T> ds;  // rounded to the type for the product: half a step each, as much as rounding dq once more
       ds.set(x);
 #pragma unroll
-      for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(kt, kb * 32, b, lane, ds, dq[b]);
+      for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(kt, kb * 32, b, at, ds, dq[b]);
     }
+  };
+  auto step = [&](int n) {
+    tiles_ready();
+    if (n + 1 < tiles) load(n + 1);
+  };
+  // (counts of tiles; the wave's queries iw .. iw + 31 lie at the keys' places + ahead)
+  Passage way = {};
+  const int whole = keys / S::KEYS;  // tiles with no row behind the last key
+  const int end = iw >= w.lq ? 0 : a.s.causal ? min(tiles, floor_div(iw + 31 + ahead, S::KEYS) + 1) : tiles;
+  way.near0 = way.near1 = way.far1 = max(end, 0);
+  if constexpr (!BIAS) {
+    way.far0 = max(0, min(end, a.s.causal ? min(whole, floor_div(iw + ahead + 1, S::KEYS)) : whole));
+    walk(way, tiles, step, [&](int n) { tile(False(), Mode<NONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); },
+         [&](int n) { tile(True(), Mode<NONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
+  } else if (a.s.pos_q) {
+    walk(way, tiles, step, [](int) {},
+         [&](int n) { tile(True(), Mode<GIVEN>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
+  } else {
+    way.far0 = max(0, min(min(end, whole), floor_div(iw + ahead - far + 1, S::KEYS)));
+    if (!a.s.causal) {
+      way.near0 = max(way.far0, min(end, -floor_div(-(far + iw + 31 + ahead), S::KEYS)));
+      way.far1 = max(way.near0, min(end, whole));
+    }
+    walk(way, tiles, step, [&](int n) { tile(False(), Mode<ONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); },
+         [&](int n) { tile(True(), Mode<NEAR>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
   }
 
   float finite = 0.0f;
@@ -187,7 +206,7 @@ __global__ __launch_bounds__(256, (DqShape<T, DP>::PER_SIMD)) void pa_dq_kernel(
           finite = fmaf(z, 0.0f, finite);
           y[e] = (T)z;
         }
-        if (valid && d < a.dim) *(t4*)((T*)a.dq + at + d) = y;
+        if (valid && d < a.dim) *(t4*)((T*)a.dq + to + d) = y;
       }
   if (sums) {
     __syncthreads();
@@ -209,8 +228,9 @@ template <typename T, int DP>
 struct DkvShape {
   static constexpr int WAVES = 4, COLS = 32 * WAVES, ROWS = sizeof(T) == 4 ? 32 : 64;
   typedef Tile<T, DP, ROWS> Tl;
-  static constexpr int BUFFER = 2 * Tl::BYTES + 4 * 256;  // q, dout, two stats, delta, positions
-  static constexpr int PER_SIMD = DP == 128 ? 1 : 2;
+  static constexpr int BUFFER = 2 * Tl::BYTES + 4 * 256;  // q, dout, delta, stats, positions
+  static constexpr int PER_SIMD = DP == 128 ? 1 : 2, UNROLL = DP == 128 || sizeof(T) == 4 ? 1 : 2;
+  static constexpr bool APART = DP * sizeof(T) >= 256;
   static int lds(bool bias, int max_distance) { return 2 * BUFFER + (bias ? (2 * max_distance + 1) * 4 : 0); }
 };
 
@@ -219,7 +239,8 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
   typedef DkvShape<T, DP> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31,
+            half = lane >> 5;
   const int group = a.heads / a.kv_heads;
   long slot;
   int g, start;
@@ -233,6 +254,7 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
   const int jg = (int)(row0 - start), jw = jg + wave * 32, j = jw + col;  // first key of workgroup, wave; lane's own
   const bool valid = j < w.lk;
   const int ahead = w.lk - w.lq;
+  const int see = a.s.causal ? ahead : 1 << 30;  // key j is seen by queries i with j <= i + see
   const int first = a.s.causal ? max(jg - ahead, 0) : 0;  // first query that sees one of the workgroup's keys
   const int tiles = jg < w.lk && first < w.lq ? (w.lq - first + S::ROWS - 1) / S::ROWS : 0;
   const int far = a.s.max_distance;
@@ -248,6 +270,24 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
 #pragma unroll
   for (int b = 0; b < Tl::BLOCKS; ++b) dk[b] = dv[b] = (f32x16)0.0f;
 
+  // (counts of tiles, from query `first` on; the wave's keys jw .. jw + 31 lie at the queries' places + ahead)
+  Passage way = {};
+  const int whole = tiles > 0 ? (w.lq - first) / S::ROWS : 0, mine = jw < w.lk ? tiles : 0;
+  const int at0 = first + ahead - jw;  // where the first query lies, seen from the wave's first key
+  way.begin = a.s.causal ? max(0, min(mine, -floor_div(at0 + S::ROWS - 1, S::ROWS))) : 0;
+  way.near0 = way.near1 = mine;
+  way.far0 = way.begin;
+  if (!BIAS) {  // hidden in part by the mask; not at all; by the last query's end
+    way.near0 = a.s.causal ? max(way.begin, min(mine, -floor_div(at0 - 31, S::ROWS))) : way.begin;
+    way.far1 = max(way.near0, min(mine, whole));
+  } else if (a.s.pos_q) {
+    way.far1 = mine;
+  } else {
+    if (!a.s.causal) way.far0 = max(way.begin, min(min(mine, whole), floor_div(-at0 - far + 1, S::ROWS)));
+    way.near0 = max(way.far0, min(mine, -floor_div(at0 - 31 - far, S::ROWS)));
+    way.far1 = max(way.near0, min(mine, whole));
+  }
+
   for (int h = g * group; h < (g + 1) * group && tiles > 0; ++h) {
     Loader<T, DP, S::ROWS, S::WAVES> lq, ld;
     lq.init((const T*)a.q + (long)w.q0 * a.q_row + h * a.q_head, a.q_row, a.dim);
@@ -260,69 +300,88 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
       lq.load(b, r, w.lq);
       ld.load(b + Tl::BYTES, r, w.lq);
       char* e = b + 2 * Tl::BYTES;
-      load_words(e, stats, r, w.lq);
-      load_words(e + 256, stats + (long)a.heads * a.nq, r, w.lq);
-      load_words(e + 512, delta, r, w.lq);
+      load_words(e, delta, r, w.lq);
+      load_words(e + 256, BIAS ? stats : delta + (long)a.heads * a.nq, r, w.lq);
+      if (BIAS) load_words(e + 512, stats + (long)a.heads * a.nq, r, w.lq);
       if (BIAS && a.s.pos_q) load_words(e + 768, a.s.pos_q + w.q0, r, w.lq);
     };
     __syncthreads();  // the last head's tiles and table are read
     load(0);
     if (BIAS) load_table(by_distance, a.s, a.table, h);
-    for (int n = 0; n < tiles; ++n) {
-      tiles_ready();
-      if (n + 1 < tiles) load(n + 1);
-      const char* qt = lds + (n & 1) * S::BUFFER;
+    typename Tl::Lane at(lane);
+    auto tile = [&](auto masked, auto mode, const char* qt, int i0) {
+      constexpr bool MASK = decltype(masked)::value;
+      constexpr int MODE = decltype(mode)::value;
       const char* dt = qt + Tl::BYTES;
-      const float* rows = (const float*)(dt + Tl::BYTES);
-      const int i0 = first + n * S::ROWS;
-      if (jw >= w.lk || (a.s.causal && jw > i0 + S::ROWS - 1 + ahead)) continue;
-#pragma unroll
+      at.fresh();
+      const float* rows = (const float*)(dt + Tl::BYTES);  // delta; ref, or m and ll; positions
+      const float one = MODE == ONE ? by_distance[jw < i0 + ahead ? 0 : 2 * far] : 0.0f;
+#pragma unroll S::UNROLL
       for (int qb = 0; qb < S::ROWS / 32; ++qb) {
-        const int ib = i0 + qb * 32;
         f32x16 x = (f32x16)0.0f, dp = (f32x16)0.0f;
 #pragma unroll
-        for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(qt, qb * 32 + col, s, half), k[s]);
+        for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(qt, qb * 32, s, at), k[s]);
+        if (S::APART) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int s = 0; s < Tl::STEPS; ++s) mma_step(dp, Tl::frag(dt, qb * 32 + col, s, half), v[s]);
-        const bool mask = ib + 32 > w.lq || (a.s.causal && jw + 31 > ib + ahead);
-        const int lo = jw - (ib + 31 + ahead), hi = jw + 31 - (ib + ahead);
-        const bool one = BIAS && !a.s.pos_q && (hi <= -far || lo >= far);
-        const float all = BIAS ? by_distance[hi <= -far ? 0 : 2 * far] : 0.0f;
+        for (int s = 0; s < Tl::STEPS; ++s) mma_step(dp, Tl::frag(dt, qb * 32, s, at), v[s]);
+        if (S::APART) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = qb * 32 + acc_row(r, half), i = i0 + row;
-          const float m = rows[row], ll = rows[64 + row] - Lift<T>::LOG2;
-          float p;
-          bool open = !mask || (i < w.lq && (!a.s.causal || j <= i + ahead));
-          if (BIAS) {
-            float e = all;
-            if (!one) {
-              const int pos_q = a.s.pos_q ? ((const int*)rows)[192 + row] : i + ahead;
-              e = by_distance[pa_entry(pa_apart(pos_k, pos_q), far)];
+        for (int t = 0; t < 4; ++t) {
+          const int row0 = qb * 32 + 8 * t + 4 * half;
+          const f32x4 delta = *(const f32x4*)(rows + row0), ref = *(const f32x4*)(rows + 64 + row0);
+          f32x4 ll;
+          i32x4 pos;
+          if (MODE != NONE) ll = *(const f32x4*)(rows + 128 + row0);
+          if (MODE == GIVEN) pos = *(const i32x4*)(rows + 192 + row0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = i0 + row0 + e, r = 4 * t + e;
+            float p;
+            int open = true;
+            if (MASK) open = (int)(i < w.lq) & (int)(j <= i + see);
+            if constexpr (MODE == NONE) {
+              p = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -ref[e]));
+            } else {
+              float b = one;
+              if (MODE == NEAR) b = by_distance[pa_entry(pos_k - (i + ahead), far)];
+              if (MODE == GIVEN) b = by_distance[pa_entry(pa_apart(pos_k, pos[e]), far)];
+              open &= (int)(b != -INFINITY);
+              p = __builtin_amdgcn_exp2f((fmaf(x[r], sc, b) - ref[e]) - (ll[e] - Lift<T>::LOG2));
             }
-            open = open && e != -INFINITY;
-            p = __builtin_amdgcn_exp2f((fmaf(x[r], sc, e) - m) - ll);
-          } else {
-            p = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -(m + ll)));
+            const float ds = p * (dp[r] - delta[e]);
+            x[r] = (!MASK && MODE == NONE) || open ? p : 0.0f;
+            dp[r] = (!MASK && MODE == NONE) || open ? ds : 0.0f;
           }
-          x[r] = open ? p : 0.0f;
-          dp[r] = open ? p * (dp[r] - rows[128 + row]) : 0.0f;
         }
         Probs<T> pp, ds;  // rounded to the type: half a step each
         pp.set(x);
         ds.set(dp);
 #pragma unroll
         for (int b = 0; b < Tl::BLOCKS; ++b) {
-          Tl::mma_t(dt, qb * 32, b, lane, pp, dv[b]);
-          Tl::mma_t(qt, qb * 32, b, lane, ds, dk[b]);
+          Tl::mma_t(dt, qb * 32, b, at, pp, dv[b]);
+          Tl::mma_t(qt, qb * 32, b, at, ds, dk[b]);
         }
       }
-    }
+    };
+    auto step = [&](int n) {
+      tiles_ready();
+      if (n + 1 < tiles) load(n + 1);
+    };
+    walk(way, tiles, step,
+         [&](int n) {
+           tile(False(), Mode<BIAS ? ONE : NONE>(), lds + (n & 1) * S::BUFFER, first + n * S::ROWS);
+         },
+         [&](int n) {
+           const char* qt = lds + (n & 1) * S::BUFFER;
+           if constexpr (!BIAS) tile(True(), Mode<NONE>(), qt, first + n * S::ROWS);
+           else if (a.s.pos_q) tile(True(), Mode<GIVEN>(), qt, first + n * S::ROWS);
+           else tile(True(), Mode<NEAR>(), qt, first + n * S::ROWS);
+         });
   }
 
   float finite = 0.0f;
   const bool there = row0 + wave * 32 + col < end;  // keys' gradients, and zeros behind a sequence's keys
-  const long at = ((row0 + wave * 32 + col) * a.kv_heads + g) * a.dim;
+  const long to = ((row0 + wave * 32 + col) * a.kv_heads + g) * a.dim;
 #pragma unroll
   for (int b = 0; b < Tl::BLOCKS; ++b)
 #pragma unroll
@@ -337,7 +396,7 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
         y[e] = valid ? (T)fk : (T)0.0f;
         z[e] = valid ? (T)fv : (T)0.0f;
       }
-      if (there && d < a.dim) *(t4*)((T*)a.dk + at + d) = y, *(t4*)((T*)a.dv + at + d) = z;
+      if (there && d < a.dim) *(t4*)((T*)a.dk + to + d) = y, *(t4*)((T*)a.dv + to + d) = z;
     }
   const unsigned long long again = __ballot(valid && !(finite == 0.0f));
   for (unsigned rows = (unsigned)again | (unsigned)(again >> 32); rows; rows &= rows - 1)
@@ -357,7 +416,7 @@ static bool launch_bwd(const PaArgs& a, hipStream_t st, bool dq, bool dkv) {
   const long slots_q = (a.nq >> 7) + a.s.batch + 2, slots_k = (a.nk >> 7) + a.s.batch + 2;
   if (dq) {
     typedef DqShape<T, DP> S;
-    if (a.table) PA_LAUNCH((pa_dq_kernel<T, DP, true>), slots_q, a.heads, S::lds(true, far, a.part ? a.s.num_buckets : 0),
+    if (a.table) PA_LAUNCH((pa_dq_kernel<T, DP, true>), slots_q, a.heads, S::lds(true, far, a.s.num_buckets),
                            S::lds(true, PA_MAX_DISTANCE, PA_MAX_BUCKETS))
     else PA_LAUNCH((pa_dq_kernel<T, DP, false>), slots_q, a.heads, S::lds(false, 0, 0), S::lds(false, 0, 0))
   }

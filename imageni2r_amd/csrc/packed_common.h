@@ -37,3 +37,10 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
     for (int i = 0; i < (int)(16 / sizeof(T)); ++i) x[c * (16 / sizeof(T)) + i] = (float)w[i];
   }
 }
+
+// fp16 holds no probability below 6e-8 and few digits below 6e-5: there p and ds carry 2^12, taken out at the end.
+template <typename T>
+struct Lift {
+  static constexpr float LOG2 = sizeof(T) == 2 && __is_same(T, f16_t) ? 12.0f : 0.0f;
+  static constexpr float DOWN = LOG2 > 0.0f ? 1.0f / 4096.0f : 1.0f;
+};

@@ -16,7 +16,8 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
   typedef FwdShape<T, DP> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31,
+            half = lane >> 5;
   long slot;
   int h, start;
   if (!tile_of(slots, a.heads, slot, h)) return;
@@ -26,9 +27,9 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
   if (span == 0 || span > a.s.batch) {  // rows of no sequence
     const int end = (int)min(row0 + S::ROWS, (long)(span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq));
     for (long i = (row0 * a.dim) + threadIdx.x; i < (long)end * a.dim; i += 256) {
-      const long at = (i / a.dim * a.heads + h) * a.dim + i % a.dim;
-      if (a.zero_outside) ((T*)a.out)[at] = (T)0.0f;
-      if (a.out32) a.out32[at] = 0.0f;
+      const long to = (i / a.dim * a.heads + h) * a.dim + i % a.dim;
+      if (a.zero_outside) ((T*)a.out)[to] = (T)0.0f;
+      if (a.out32) a.out32[to] = 0.0f;
     }
     return;
   }
@@ -70,81 +71,106 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
   for (int b = 0; b < Tl::BLOCKS; ++b) o[b] = (f32x16)0.0f;
   float m = -INFINITY, l = 0.0f;  // the column's reference exponent; the lane's half of the sum
 
-  for (int n = 0; n < tiles; ++n) {
-    tiles_ready();
-    if (n + 1 < tiles) load(n + 1);
-    const char* kt = lds + (n & 1) * S::BUFFER;
+  // One tile.  MASK: some pairs may be hidden by their place; MODE: where the bias comes from.
+  typename Tl::Lane at(lane);
+  auto tile = [&](auto masked, auto mode, const char* kt, int j0) {
+    constexpr bool MASK = decltype(masked)::value;
+    constexpr int MODE = decltype(mode)::value, BLOCKS = S::KEYS / 32;
     const char* vt = kt + Tl::BYTES;
-    const int j0 = n * S::KEYS;
-    if (iw >= w.lq || (a.s.causal && j0 > iw + 31 + ahead)) continue;  // nothing for this wave
+    at.fresh();
+    f32x16 x[BLOCKS];
 #pragma unroll
-    for (int kb = 0; kb < S::KEYS / 32; ++kb) {
-      const int jb = j0 + kb * 32;
-      f32x16 x = (f32x16)0.0f;
+    for (int kb = 0; kb < BLOCKS; ++kb) {
+      x[kb] = (f32x16)0.0f;
 #pragma unroll
-      for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(kt, kb * 32 + col, s, half), q[s]);
-      if (BIAS) {
-        const int lo = jb - (iw + 31 + ahead), hi = jb + 31 - (iw + ahead);  // smallest and largest distance
-        if (!a.s.pos_q && (hi <= -far || lo >= far)) {
-          const float b = by_distance[hi <= -far ? 0 : 2 * far];
+      for (int s = 0; s < Tl::STEPS; ++s) mma_step(x[kb], Tl::frag(kt, kb * 32, s, at), q[s]);
+    }
+    const float one = MODE == ONE ? by_distance[j0 < iw + ahead ? 0 : 2 * far] : 0.0f;
+    const int last = a.s.causal ? min(keys, i + ahead + 1) : keys;  // keys the lane's query sees
+    float top = -INFINITY;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], sc, b);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int row = acc_row(r, half);
-            const int pos_k = a.s.pos_k ? ((const int*)(vt + Tl::BYTES))[kb * 32 + row] : jb + row;
-            x[r] = fmaf(x[r], sc, by_distance[pa_entry(pa_apart(pos_k, pos_q), far)]);
-          }
-        }
-      }
-      const int last = a.s.causal ? min(keys, i + ahead + 1) : keys;  // keys the lane's query sees
-      if (jb + 32 > keys || (a.s.causal && jb + 31 > iw + ahead)) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = jb + acc_row(r, half) < last ? x[r] : -INFINITY;
-      }
-      float top = x[0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
-      top = fmaxf(top, other_half(top));
-      if (!BIAS) top *= sc;
-      // The reference exponent moves only when a score passes it by 2^8: the sums stay far from overflow, and most
-      // blocks rescale nothing.
-      if (__any(top > m + 8.0f || m == -INFINITY)) {
-        const float mn = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        l *= fall;
-#pragma unroll
-        for (int b = 0; b < Tl::BLOCKS; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[b][r] *= fall;
-        m = mn;
-      }
-      const float ref = m == -INFINITY ? 0.0f : m;
+    for (int kb = 0; kb < BLOCKS; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        x[r] = __builtin_amdgcn_exp2f(BIAS ? x[r] - ref : fmaf(x[r], sc, -ref));
-        l += x[r];
+        const int row = kb * 32 + acc_row(r, half);
+        float y = x[kb][r];
+        if (MODE == ONE) y = fmaf(y, sc, one);
+        if (MODE == NEAR) y = fmaf(y, sc, by_distance[pa_entry(j0 + row - pos_q, far)]);
+        if (MODE == GIVEN)
+          y = fmaf(y, sc, by_distance[pa_entry(pa_apart(((const int*)(vt + Tl::BYTES))[row], pos_q), far)]);
+        if (MASK) y = j0 + row < last ? y : -INFINITY;
+        x[kb][r] = y;
+        top = fmaxf(top, y);
+      }
+    top = fmaxf(top, other_half(top));
+    if (!BIAS) top *= sc;
+    // The reference exponent moves only when a score passes it by 2^8: the sums stay far from overflow, and most tiles
+    // rescale nothing.
+    if (__any(top > m + 8.0f || m == -INFINITY)) {
+      const float mn = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      l *= fall;
+#pragma unroll
+      for (int b = 0; b < Tl::BLOCKS; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[b][r] *= fall;
+      m = mn;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int kb = 0; kb < BLOCKS; ++kb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        x[kb][r] = __builtin_amdgcn_exp2f(BIAS ? x[kb][r] - ref : fmaf(x[kb][r], sc, -ref));
+        l += x[kb][r];
       }
       // Rounding the probabilities to the type puts each off by at most half a step, independently: as much as rounding
       // the output once more.  The table's gradient is fp32, and delta = <dout, out> enters it: with a bias to train
-      // the rounded-away rest is multiplied too.
+      // what the rounding took away is multiplied too, until 22 bits (fp16) or 24 (bf16) of each have been.
       Probs<T> p;
-      p.set(x);
-#pragma unroll
-      for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(vt, kb * 32, b, lane, p, o[b]);
       if constexpr (BIAS && SAVE && sizeof(T) == 2) {
-        Probs<T> rest;
-        rest.set_rest(x, p);
 #pragma unroll
-        for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(vt, kb * 32, b, lane, rest, o[b]);
+        for (int part = 0; part < (__is_same(T, f16_t) ? 2 : 3); ++part) {
+          p.set_and_take(x[kb]);
+#pragma unroll
+          for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(vt, kb * 32, b, at, p, o[b]);
+        }
+      } else {
+        p.set(x[kb]);
+#pragma unroll
+        for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(vt, kb * 32, b, at, p, o[b]);
       }
     }
+  };
+  auto step = [&](int n) {
+    tiles_ready();
+    if (n + 1 < tiles) load(n + 1);
+  };
+  // (counts of tiles; the wave's queries iw .. iw + 31 lie at the keys' places + ahead)
+  Passage way = {};
+  const int whole = keys / S::KEYS;  // tiles with no row behind the last key
+  const int end = iw >= w.lq ? 0 : a.s.causal ? min(tiles, floor_div(iw + 31 + ahead, S::KEYS) + 1) : tiles;
+  way.near0 = way.near1 = way.far1 = max(end, 0);
+  if constexpr (!BIAS) {
+    way.far0 = max(0, min(end, a.s.causal ? min(whole, floor_div(iw + ahead + 1, S::KEYS)) : whole));
+    walk(way, tiles, step, [&](int n) { tile(False(), Mode<NONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); },
+         [&](int n) { tile(True(), Mode<NONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
+  } else if (a.s.pos_q) {
+    walk(way, tiles, step, [](int) {},
+         [&](int n) { tile(True(), Mode<GIVEN>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
+  } else {
+    way.far0 = max(0, min(min(end, whole), floor_div(iw + ahead - far + 1, S::KEYS)));
+    if (!a.s.causal) {
+      way.near0 = max(way.far0, min(end, -floor_div(-(far + iw + 31 + ahead), S::KEYS)));
+      way.far1 = max(way.near0, min(end, whole));
+    }
+    walk(way, tiles, step, [&](int n) { tile(False(), Mode<ONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); },
+         [&](int n) { tile(True(), Mode<NEAR>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
   }
 
   l += other_half(l);
   const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
   float finite = l * 0.0f;
-  const long at = ((long)(w.q0 + i) * a.heads + h) * a.dim;
+  const long to = ((long)(w.q0 + i) * a.heads + h) * a.dim;
 #pragma unroll
   for (int b = 0; b < Tl::BLOCKS; ++b)
 #pragma unroll
@@ -160,8 +186,8 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
         y[e] = (T)z[e];
       }
       if (valid && d < a.dim) {
-        *(t4*)((T*)a.out + at + d) = y;
-        if (SAVE && sizeof(T) == 2 && a.out32) *(f32x4*)(a.out32 + at + d) = z;
+        *(t4*)((T*)a.out + to + d) = y;
+        if (SAVE && sizeof(T) == 2 && a.out32) *(f32x4*)(a.out32 + to + d) = z;
       }
     }
   if (SAVE && valid && half == 0) {

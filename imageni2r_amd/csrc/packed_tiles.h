@@ -8,6 +8,7 @@
 // block, and A's transposed fragments are read from LDS in that same order.
 #pragma once
 #include "packed_rows.h"
+#include <type_traits>
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -45,38 +46,55 @@ struct Tile {
   static constexpr int STEPS = ROW_BYTES / 32;  // steps of a product over the head dim
   static constexpr int BLOCKS = DP / 32;        // 32-wide blocks of the head dim
 
-  __device__ static __forceinline__ int swizzle(int row) {
+  // (made of the row's bits by exclusive or: what two disjoint sets of bits give is the exclusive or of both)
+  __host__ __device__ static constexpr int swizzle(int row) {
     return CHUNKS >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : CHUNKS == 8 ? ((row & 1) << 2) | ((row >> 1) & 3) : (row >> 1) & 3;
   }
-  __device__ static __forceinline__ int at(int row, int chunk) { return row * ROW_BYTES + ((chunk ^ swizzle(row)) << 4); }
 
-  // fragment of row `row` (the lane's own) for step s
-  __device__ static __forceinline__ frag_t<T> frag(const char* tile, int row, int s, int h) {
-    return *(const frag_t<T>*)(tile + at(row, 2 * s + h));
+  // A lane's two places in a block of 32 rows, from which every other differs by constants.  fresh() keeps the compiler
+  // from holding all those sums in registers across tiles: at a head dim of 128 they are what would spill.
+  struct Lane {
+    int f, t;
+    __device__ __forceinline__ explicit Lane(int lane) {
+      const int half = lane >> 5, col = lane & 31;
+      f = col * ROW_BYTES + ((half ^ swizzle(col)) << 4);
+      if (sizeof(T) == 4) {
+        t = 4 * half * ROW_BYTES + (((col >> 2) ^ swizzle(4 * half)) << 4) + (col & 3) * 4;
+      } else {
+        const int n = lane & 15, row = 4 * half + (n >> 2), chunk = ((lane >> 4) & 1) * 2 + ((n & 3) >> 1);
+        t = row * ROW_BYTES + ((chunk ^ swizzle(row)) << 4) + (n & 1) * 8;
+      }
+    }
+    __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(f), "+v"(t)); }
+  };
+
+  // the lane's row of the 32 from r0 on, step s
+  __device__ static __forceinline__ frag_t<T> frag(const char* tile, int r0, int s, const Lane& at) {
+    return *(const frag_t<T>*)(tile + r0 * ROW_BYTES + (at.f ^ (s << 5)));
   }
 
   // acc[32 d of block db][columns] += tile(rows r0 .. r0 + 32)^T p, p the accumulators of those rows
   template <typename P>
-  __device__ static __forceinline__ void mma_t(const char* tile, int r0, int db, int lane, const P& p, f32x16& acc) {
-    const int h = lane >> 5;
+  __device__ static __forceinline__ void mma_t(const char* tile, int r0, int db, const Lane& at, const P& p, f32x16& acc) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int d = db * 32 + (lane & 31), row = r0 + acc_row(r, h);
-        const float a = *(const float*)(tile + at(row, d >> 2) + (d & 3) * 4);
+        const int row = acc_row(r, 0);
+        const float a = *(const float*)(tile + (r0 + row) * ROW_BYTES + (at.t ^ (db << 7) ^ (swizzle(row) << 4)));
         acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc, 0, 0, 0);
       }
     } else {
-      // ds_read_b64_tr_b16: of each 16 lanes, lane t addresses 4 elements of row t >> 2, and gets column t of the 4 rows
-      const int t = lane & 15, row = r0 + 4 * h + (t >> 2);
-      const int chunk = db * 4 + ((lane >> 4) & 1) * 2 + ((t & 3) >> 1);
+      // ds_read_b64_tr_b16: of each 16 lanes, lane n addresses 4 elements of row n >> 2, and gets column n of the 4 rows
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            LDS_PTR(s16x4, (char*)tile + at(row + 16 * c, chunk) + (t & 1) * 8));
-        s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            LDS_PTR(s16x4, (char*)tile + at(row + 16 * c + 8, chunk) + (t & 1) * 8));
-        const s16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        s16x4 part[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = 16 * c + 8 * e;
+          part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              LDS_PTR(s16x4, (char*)tile + (r0 + row) * ROW_BYTES + (at.t ^ (db << 6) ^ (swizzle(row) << 4))));
+        }
+        const s16x8 a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
         mma_step(acc, __builtin_bit_cast(frag_t<T>, a), p[c]);
       }
     }
@@ -92,10 +110,11 @@ struct Probs {
 #pragma unroll
     for (int r = 0; r < 16; ++r) f[r >> 3][r & 7] = (T)x[r];
   }
-  // what set() rounded away
-  __device__ __forceinline__ void set_rest(const f32x16& x, const Probs& first) {
+  // what the rounding took away is left in x
+  __device__ __forceinline__ void set_and_take(f32x16& x) {
+    set(x);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) f[r >> 3][r & 7] = (T)(x[r] - (float)first.f[r >> 3][r & 7]);
+    for (int r = 0; r < 16; ++r) x[r] -= (float)f[r >> 3][r & 7];
   }
 };
 template <>
@@ -189,6 +208,43 @@ __device__ __forceinline__ void load_words(void* to, const void* from, int first
                :
                : "s"(lds), "v"((int)threadIdx.x * 4), "s"(rs)
                : "memory");
+}
+
+// Where a tile's bias comes from: there is none; all distances lie beyond max_distance on one side; places in the sequence;
+// positions that the caller gave.
+enum { NONE, ONE, NEAR, GIVEN };
+template <int M>
+using Mode = std::integral_constant<int, M>;
+using True = std::true_type;
+using False = std::false_type;
+
+__device__ __forceinline__ int floor_div(int a, int b) { return a >= 0 ? a / b : -((b - 1 - a) / b); }
+
+// The tiles of a pass over keys (or queries), as one wave meets them: [0, begin) none of its pairs; then in turn tiles
+// whose distances are all beyond max_distance (one bias, nothing hidden) up to far0, others up to near0, and so again up to
+// far1 and near1; behind that none.  One loop for each kind, so that the accumulators stay where they are; every wave passes every tile's
+// barrier, whichever loop it is in.
+struct Passage {
+  int begin, far0, near0, far1, near1;
+};
+template <typename Step, typename Far, typename Near>
+__device__ __forceinline__ void walk(const Passage& p, int tiles, Step step, Far far_tile, Near near_tile) {
+  int n = 0;
+  for (; n < p.begin; ++n) step(n);
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll 1
+    for (; n < (k ? p.far1 : p.far0); ++n) {
+      step(n);
+      far_tile(n);
+    }
+#pragma unroll 1
+    for (; n < (k ? p.near1 : p.near0); ++n) {
+      step(n);
+      near_tile(n);
+    }
+  }
+  for (; n < tiles; ++n) step(n);
 }
 
 // Order of the tiles: each of the 8 XCDs (workgroups go to them in turn) works through whole heads, so that what a head's

@@ -44,11 +44,11 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>
     const int end = span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq;
     const int row = row0 + token;
     if (split || wave || half || !column || row >= end) return;
-    const long at = ((long)row * a.heads + h) * a.dim;
+    const long to = ((long)row * a.heads + h) * a.dim;
     if (p.splits > 1) p.ml[parts + (long)row * a.heads + h] = -1.0f;  // l < 0: no sequence's
     for (int d = 0; d < a.dim; ++d) {
-      if (a.zero_outside) ((T*)a.out)[at + d] = (T)0.0f;
-      if (a.out32) a.out32[at + d] = 0.0f;
+      if (a.zero_outside) ((T*)a.out)[to + d] = (T)0.0f;
+      if (a.out32) a.out32[to + d] = 0.0f;
     }
     return;
   }
@@ -101,6 +101,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>
 #pragma unroll
   for (int b = 0; b < Tl::BLOCKS; ++b) o[b] = (f32x16)0.0f;
   float m = -INFINITY, l = 0.0f;
+  const typename Tl::Lane at(lane);
   for (int n = 0, b = b0 + wave; b < b1; ++n, b += S::WAVES) {
     if (b + S::WAVES < b1) {
       load(n + 1, b + S::WAVES);
@@ -113,7 +114,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>
     const int jb = b * 32;
     f32x16 x = (f32x16)0.0f;
 #pragma unroll
-    for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(kt, col, s, half), q[s]);
+    for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(kt, 0, s, at), q[s]);
     if (BIAS) {
       const int hi = jb + 31 - (i0 + ahead);  // largest distance
       if (!a.s.pos_q && hi <= -far) {
@@ -154,17 +155,20 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>
       x[r] = __builtin_amdgcn_exp2f(BIAS ? x[r] - ref : fmaf(x[r], sc, -ref));
       l += x[r];
     }
-    Probs<T> pr;  // rounded to the type: half a step each, as much as rounding the output once more
-    pr.set(x);
-#pragma unroll
-    for (int t = 0; t < Tl::BLOCKS; ++t) Tl::mma_t(vt, 0, t, lane, pr, o[t]);
+    // rounded to the type: half a step each, as much as rounding the output once more; with a table to train (delta enters
+    // its fp32 gradient) what the rounding took away is multiplied too
+    Probs<T> pr;
     if constexpr (BIAS && sizeof(T) == 2) {
-      if (a.stats) {  // delta enters the table's fp32 gradient: what the rounding took away is multiplied too
-        Probs<T> more;
-        more.set_rest(x, pr);
+      const int terms = !a.stats ? 1 : __is_same(T, f16_t) ? 2 : 3;
+      for (int part = 0; part < terms; ++part) {
+        pr.set_and_take(x);
 #pragma unroll
-        for (int t = 0; t < Tl::BLOCKS; ++t) Tl::mma_t(vt, 0, t, lane, more, o[t]);
+        for (int t = 0; t < Tl::BLOCKS; ++t) Tl::mma_t(vt, 0, t, at, pr, o[t]);
       }
+    } else {
+      pr.set(x);
+#pragma unroll
+      for (int t = 0; t < Tl::BLOCKS; ++t) Tl::mma_t(vt, 0, t, at, pr, o[t]);
     }
   }
   l += other_half(l);
