@@ -8,7 +8,7 @@ struct FwdShape {
   static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
   typedef Tile<T, DP, KEYS> Tl;
   static constexpr int BUFFER = 2 * Tl::BYTES + 256;  // k, v, positions
-  static int lds(bool bias, int max_distance) { return 2 * BUFFER + (bias ? (2 * max_distance + 1) * 4 : 0); }
+  static int lds(bool bias, int max_distance) { return 2 * BUFFER + (bias ? table_places(max_distance) * 4 : 0); }
 };
 
 template <typename T, int DP, bool BIAS, bool SAVE>
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
 
   // One tile.  MASK: some pairs may be hidden by their place; MODE: where the bias comes from.
   typename Tl::Lane at(lane);
-  auto tile = [&](auto masked, auto mode, const char* kt, int j0) {
+  auto tile = [&](auto masked, auto mode, const char* kt, int j0) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(masked)::value;
     constexpr int MODE = decltype(mode)::value, BLOCKS = S::KEYS / 32;
     const char* vt = kt + Tl::BYTES;
@@ -85,7 +85,9 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
 #pragma unroll
       for (int s = 0; s < Tl::STEPS; ++s) mma_step(x[kb], Tl::frag(kt, kb * 32, s, at), q[s]);
     }
-    const float one = MODE == ONE ? by_distance[j0 < iw + ahead ? 0 : 2 * far] : 0.0f;
+    const float one = MODE == ONE ? by_distance[j0 < iw + ahead ? 0 : 2 * (far + PAD)] : 0.0f;
+    // the place of the tile's first row (clamped so far out that all rows' places are beyond max_distance)
+    const float* near = by_distance + (min(max(j0 + 4 * half - pos_q, -far - 60), far) + far + PAD);
     const int last = a.s.causal ? min(keys, i + ahead + 1) : keys;  // keys the lane's query sees
     float top = -INFINITY;
 #pragma unroll
@@ -95,9 +97,9 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
         const int row = kb * 32 + acc_row(r, half);
         float y = x[kb][r];
         if (MODE == ONE) y = fmaf(y, sc, one);
-        if (MODE == NEAR) y = fmaf(y, sc, by_distance[pa_entry(j0 + row - pos_q, far)]);
+        if (MODE == NEAR) y = fmaf(y, sc, near[kb * 32 + acc_row(r, 0)]);
         if (MODE == GIVEN)
-          y = fmaf(y, sc, by_distance[pa_entry(pa_apart(((const int*)(vt + Tl::BYTES))[row], pos_q), far)]);
+          y = fmaf(y, sc, by_distance[PAD + pa_entry(pa_apart(((const int*)(vt + Tl::BYTES))[row], pos_q), far)]);
         if (MASK) y = j0 + row < last ? y : -INFINITY;
         x[kb][r] = y;
         top = fmaxf(top, y);

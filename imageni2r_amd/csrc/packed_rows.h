@@ -10,8 +10,8 @@ struct PaArgs {
   const void *q, *k, *v, *dout;
   const float *table, *out32_in;
   void *out, *dq, *dk, *dv;
-  float *out32, *stats, *delta, *part;
-  int nq, nk, heads, kv_heads, dim, zero_outside;
+  float *out32, *stats, *delta, *part, *dkv_part;
+  int nq, nk, heads, kv_heads, dim, zero_outside, parts;
   long q_row, q_head, k_row, k_head, v_row, v_head;
   float scale;
 };
@@ -33,6 +33,14 @@ __device__ __forceinline__ int pa_span(const int* cu, int batch, int n, int shif
   }
   start = count == 1 ? 0 : pa_clamp(cu[count - 2], n);
   return count - 1;
+}
+
+// the sequence that a row (of some sequence) belongs to: the last that starts at or before it (every lane of the wave calls)
+__device__ __forceinline__ int pa_seq_of(const int* cu, int batch, int n, int row) {
+  const int lane = threadIdx.x & 63;
+  int count = 0;
+  for (int i0 = 0; i0 < batch; i0 += 64) count += __popcll(__ballot(i0 + lane < batch && pa_clamp(cu[i0 + lane], n) <= row));
+  return max(count - 1, 0);
 }
 
 struct PaSeq {

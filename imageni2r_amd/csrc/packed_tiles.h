@@ -14,7 +14,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-#define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
+// (the low half of a flat address is the place in LDS; the plain cast would test it for null)
+#define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(unsigned)(uintptr_t)(p))
 
 // row of the block that accumulator r of lane half h holds
 __device__ __forceinline__ constexpr int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
@@ -227,10 +228,14 @@ __device__ __forceinline__ int floor_div(int a, int b) { return a >= 0 ? a / b :
 struct Passage {
   int begin, far0, near0, far1, near1;
 };
-template <typename Step, typename Far, typename Near>
-__device__ __forceinline__ void walk(const Passage& p, int tiles, Step step, Far far_tile, Near near_tile) {
+template <typename Step, typename Far, typename Near, typename Idle>
+__device__ __forceinline__ void walk(const Passage& p, int tiles, Step step, Far far_tile, Near near_tile, Idle idle) {
   int n = 0;
-  for (; n < p.begin; ++n) step(n);
+#pragma unroll 1
+  for (; n < p.begin; ++n) {
+    step(n);
+    idle();
+  }
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
 #pragma unroll 1
@@ -244,7 +249,15 @@ __device__ __forceinline__ void walk(const Passage& p, int tiles, Step step, Far
       near_tile(n);
     }
   }
-  for (; n < tiles; ++n) step(n);
+#pragma unroll 1
+  for (; n < tiles; ++n) {
+    step(n);
+    idle();
+  }
+}
+template <typename Step, typename Far, typename Near>
+__device__ __forceinline__ void walk(const Passage& p, int tiles, Step step, Far far_tile, Near near_tile) {
+  walk(p, tiles, step, far_tile, near_tile, [] {});
 }
 
 // Order of the tiles: each of the 8 XCDs (workgroups go to them in turn) works through whole heads, so that what a head's
@@ -258,8 +271,23 @@ __device__ __forceinline__ bool tile_of(long slots, int heads, long& slot, int& 
 }
 static inline unsigned tile_grid(long slots, int heads) { return (unsigned)((slots * heads + 7) / 8 * 8); }
 
-// One head's bias by distance, in log2 units.
+// One head's bias by distance, in log2 units, and the bucket beside it where it is wanted.  64 places more on both sides
+// hold what lies beyond max_distance, so that the places of a tile's pairs follow from one of them by constants.
+constexpr int PAD = 64;
+struct Entry {
+  float bias;
+  int bucket;
+};
+static __host__ __device__ constexpr int table_places(int max_distance) { return 2 * (max_distance + PAD) + 1; }
 __device__ __forceinline__ void load_table(float* by_distance, const i2r_packed_seqs& s, const float* table, int h) {
-  for (int n = threadIdx.x; n <= 2 * s.max_distance; n += blockDim.x)
-    by_distance[n] = pa_log2_units(table[(long)h * s.num_buckets + min((int)s.lut[n], s.num_buckets - 1)]);
+  for (int n = threadIdx.x; n < table_places(s.max_distance); n += blockDim.x) {
+    const int b = min((int)s.lut[min(max(n - PAD, 0), 2 * s.max_distance)], s.num_buckets - 1);
+    by_distance[n] = pa_log2_units(table[(long)h * s.num_buckets + b]);
+  }
+}
+__device__ __forceinline__ void load_table(Entry* by_distance, const i2r_packed_seqs& s, const float* table, int h) {
+  for (int n = threadIdx.x; n < table_places(s.max_distance); n += blockDim.x) {
+    const int b = min((int)s.lut[min(max(n - PAD, 0), 2 * s.max_distance)], s.num_buckets - 1);
+    by_distance[n] = {pa_log2_units(table[(long)h * s.num_buckets + b]), b};
+  }
 }

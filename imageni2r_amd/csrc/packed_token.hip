@@ -298,11 +298,7 @@ __global__ __launch_bounds__(256) void pa_token_join_kernel(PaArgs a, TokenPlan 
   }
   __syncthreads();
   if (mark && t < 64) {
-    // the last sequence that starts at or before the row
-    int count = 0;
-    for (int k = 0; k < a.s.batch; k += 64)
-      count += __popcll(__ballot(k + t < a.s.batch && pa_clamp(a.s.cu_q[k + t], a.nq) <= row));
-    const PaSeq w = pa_seq(a.s, a.nq, a.nk, max(count - 1, 0));
+    const PaSeq w = pa_seq(a.s, a.nq, a.nk, pa_seq_of(a.s.cu_q, a.s.batch, a.nq, row));
     if (row >= w.q0 && row < w.q0 + w.lq) pa_row_fwd<T>(a, w, row - w.q0, h);
   }
 }
