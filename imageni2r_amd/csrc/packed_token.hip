@@ -243,41 +243,64 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>
     if (marks[c]) pa_row_fwd<T>(a, w, i0 + c / p.heads, g * group + chunk * p.heads + c % p.heads);
 }
 
-// One workgroup joins the splits of one (row, head): 256 / (dim / 4) of them at a time.
+// One workgroup joins the splits of one (row, head): as many of them side by side as its threads (dim / 4 a split) allow, eight
+// of a thread's at a time -- a chain of latencies is what this costs.
 template <typename T>
-__global__ __launch_bounds__(256) void pa_token_join_kernel(PaArgs a, TokenPlan p) {
-  __shared__ f32x4 sums[256];
-  __shared__ float tops[256], ls[256];
+__global__ __launch_bounds__(1024) void pa_token_join_kernel(PaArgs a, TokenPlan p) {
+  __shared__ f32x4 sums[1024];
+  __shared__ float ls[1024], tops[16];
   __shared__ int mark;
   const long parts = (long)a.nq * a.heads, rh = blockIdx.x;
   const int row = (int)(rh / a.heads), h = (int)(rh % a.heads);
-  const int quads = a.dim / 4, lanes = 256 / quads, t = threadIdx.x, q = t % quads, n = t / quads;
-  const float first = p.ml[parts + rh];
-  if (first < 0.0f) return;  // no sequence's row: done before
+  const int quads = a.dim / 4, lanes = blockDim.x / quads, t = threadIdx.x, q = t % quads, n = t / quads;
+  if (p.ml[parts + rh] < 0.0f) return;  // no sequence's row: done before
   if (t == 0) mark = 0;
   float top = -INFINITY;
-  for (int s = t; s < p.splits; s += 256) top = fmaxf(top, p.ml[2 * s * parts + rh]);
-  tops[t] = wave_max(top);
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[64]), fmaxf(tops[128], tops[192]));
+  for (int s = t; s < p.splits; s += blockDim.x) top = fmaxf(top, p.ml[2 * s * parts + rh]);
   f32x4 z = (f32x4)0.0f;
-  float l = 0.0f;
-  if (n < lanes)
-#pragma unroll 4
-    for (int s = n; s < p.splits; s += lanes) {
-      const float m = p.ml[2 * s * parts + rh];
-      if (m == -INFINITY) continue;
-      const float fall = __builtin_amdgcn_exp2f(m - top);
-      l = fmaf(p.ml[(2 * s + 1) * parts + rh], fall, l);
-      const f32x4 o = *(const f32x4*)(p.o + (s * parts + rh) * a.dim + 4 * q);
+  float l = 0.0f, m[8];
+  f32x4 o[8];
+  auto load = [&](int s0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = fmaf(o[e], fall, z[e]);
+    for (int u = 0; u < 8; ++u) {
+      const int s = s0 + u * lanes;
+      m[u] = n < lanes && s < p.splits ? p.ml[2 * s * parts + rh] : -INFINITY;
+      o[u] = (f32x4)0.0f;
+      if (m[u] != -INFINITY) o[u] = *(const f32x4*)(p.o + (s * parts + rh) * a.dim + 4 * q);
     }
+  };
+  load(n);
+  top = wave_max(top);
+  if ((t & 63) == 0) tops[t >> 6] = top;
+  __syncthreads();
+  top = tops[0];
+  for (int v = 1; v < (int)blockDim.x / 64; ++v) top = fmaxf(top, tops[v]);
+  for (int s0 = n;;) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float fall = m[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[u] - top);
+      l = fmaf(m[u] == -INFINITY ? 0.0f : p.ml[(2 * (s0 + u * lanes) + 1) * parts + rh], fall, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = fmaf(o[u][e], fall, z[e]);
+    }
+    if ((s0 += 8 * lanes) >= p.splits) break;
+    load(s0);
+  }
   sums[t] = z;
   ls[t] = l;
   __syncthreads();
+  for (int count = lanes; count > 1;) {
+    const int keep = (count + 1) / 2;
+    if (n + keep < count) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[t][e] += sums[t + keep * quads][e];
+      ls[t] += ls[t + keep * quads];
+    }
+    __syncthreads();
+    count = keep;
+  }
   if (t < quads) {
-    for (int v = 1; v < lanes; ++v) z += sums[v * quads + t], l += ls[v * quads + t];
+    z = sums[t], l = ls[t];
     const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
     typedef T t4 __attribute__((ext_vector_type(4)));
     t4 y;
@@ -341,8 +364,10 @@ static bool launch_token(const PaArgs& a, const TokenPlan& p, hipStream_t st) {
     if (!i2r_lds_attr((const void*)pa_token_kernel<T, DP, false>, S::lds(false, 0), done[0])) return false;
     hipLaunchKernelGGL((pa_token_kernel<T, DP, false>), grid, dim3(64 * S::WAVES), S::lds(false, 0), st, a, p);
   }
-  if (p.splits > 1)
-    hipLaunchKernelGGL(pa_token_join_kernel<T>, dim3((unsigned)((long)a.nq * a.heads)), dim3(256), 0, st, a, p);
+  if (p.splits > 1) {
+    const int threads = std::min(1024, (std::min(p.splits, 128) * (a.dim / 4) + 63) / 64 * 64);
+    hipLaunchKernelGGL(pa_token_join_kernel<T>, dim3((unsigned)((long)a.nq * a.heads)), dim3(threads), 0, st, a, p);
+  }
   return true;
 }
 
