@@ -5,7 +5,8 @@ bool pa_launch_fwd(int dtype, const PaArgs& a, hipStream_t st);  // packed_fwd.h
 bool pa_is_token(int batch, int nq, int heads, int kv_heads);  // packed_token.hip
 long pa_token_ws_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim);
 bool pa_launch_token(int dtype, const PaArgs& a, void* ws, hipStream_t st);
-bool pa_launch_bwd(int dtype, const PaArgs& a, hipStream_t st, bool dq, bool dkv);  // packed_bwd.hip
+bool pa_launch_dq(int dtype, const PaArgs& a, hipStream_t st);   // packed_dq.hip
+bool pa_launch_dkv(int dtype, const PaArgs& a, hipStream_t st);  // packed_dkv.hip
 
 // delta = <dout, out> of each row and head, and the sum of its stats: for dk and dv without dq.  Two threads for each, in the
 // dq kernel's order, so that the gradients do not depend on which of them are asked for.
@@ -144,7 +145,8 @@ extern "C" int i2r_packed_attention_bwd(const i2r_packed_seqs* seqs, const void*
     else if (dtype == 1) hipLaunchKernelGGL(pa_delta_kernel<f16_t>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(pa_delta_kernel<bf16_t>, grid, dim3(256), 0, st, a);
   }
-  if (!pa_launch_bwd(dtype, a, st, need_dq, need_dkv)) return I2R_ERR_HIP;
+  if (need_dq && !pa_launch_dq(dtype, a, st)) return I2R_ERR_HIP;
+  if (need_dkv && !pa_launch_dkv(dtype, a, st)) return I2R_ERR_HIP;
   if (dtable)
     hipLaunchKernelGGL(pa_dtable_kernel, dim3(heads, nb), dim3(256), 0, st, a.part, dtable, nq ? q_slots(nq, seqs->batch) : 0,
                        heads, nb);

@@ -1,239 +1,5 @@
-// Backward of packed-sequence attention on the matrix cores.
-//
-// Two kernels, both recomputing the scores: dq (a query a column, keys pass by) and dk / dv (a key a column, the queries of
-// all heads of its group pass by).  Seven products where five would do with dq added up atomically -- but no float is ever
-// added in an order that could change, and nothing but the outputs is written.
+// Backward of packed-sequence attention on the matrix cores: dk and dv (packed_dq.hip has the other half).
 #include "packed_tiles.h"
-
-// Adds four keys' ds to the lane's column of the histogram, those of one bucket first: neighbours mostly share one, and a
-// read, an addition and a write cost the LDS less than ds_add_f32 (192 cycles an instruction of 64 lanes, measured,
-// against 7 for the integer one).  No other lane touches the column, so nothing has to be atomic.
-__device__ __forceinline__ void add_four(float* mine, const Entry* e, const float* x) {
-  const int b0 = e[0].bucket, b1 = e[1].bucket, b2 = e[2].bucket, b3 = e[3].bucket;
-  const int same1 = b1 == b0, same2 = b2 == b0, same3 = b3 == b0;
-  const int last1 = (b1 == b3) & ~same1, last2 = (b2 == b3) & ~same2;
-  const float s0 = ((x[0] + (same1 ? x[1] : 0.0f)) + (same2 ? x[2] : 0.0f)) + (same3 ? x[3] : 0.0f);
-  const float s3 = (x[3] + (last1 ? x[1] : 0.0f)) + (last2 ? x[2] : 0.0f);
-  const float h0 = mine[b0 * 64], h3 = mine[b3 * 64];
-  mine[b0 * 64] = h0 + s0;
-  if (!same3) mine[b3 * 64] = h3 + s3;
-  const int alone1 = !(same1 | last1), alone2 = !(same2 | last2);
-  if (__any(alone1 | alone2)) {
-    if (alone1) mine[b1 * 64] += x[1];
-    if (alone2) mine[b2 * 64] += x[2];
-  }
-}
-
-template <typename T, int DP>
-struct DqShape {
-  static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
-  typedef Tile<T, DP, KEYS> Tl;
-  static constexpr int BUFFER = 2 * Tl::BYTES + 256;  // k, v, positions
-  static constexpr int PER_SIMD = sizeof(T) == 4 && DP == 128 ? 1 : 2, UNROLL = DP == 128 ? 1 : 2;
-  static constexpr bool APART = DP == 128;  // the products' operands would not fit the registers all at once
-  static int lds(bool bias, int max_distance, int buckets) {
-    return 2 * BUFFER + (bias ? table_places(max_distance) * 8 + buckets * 64 * 4 * WAVES : 0);
-  }
-};
-
-// dq of 32 queries a wave, delta = <dout, out> and the two stats' sum on the way for the other kernel, and ds summed by bucket: each lane its own column of a histogram
-// in LDS, so that no two lanes add to one word.
-template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, (DqShape<T, DP>::PER_SIMD)) void pa_dq_kernel(PaArgs a, long slots) {
-  typedef DqShape<T, DP> S;
-  typedef typename S::Tl Tl;
-  extern __shared__ __align__(16) char lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31,
-            half = lane >> 5;
-  long slot;
-  int h, start;
-  if (!tile_of(slots, a.heads, slot, h)) return;
-  slot = slots - 1 - slot;
-  const bool sums = BIAS && a.part;
-  const int nb = a.s.num_buckets;
-  const int span = pa_span(a.s.cu_q, a.s.batch, a.nq, 7, slot, start);
-  const long row0 = start + ((slot - (start >> 7) - span) << 7);
-  PaSeq w = {};
-  if (span > 0 && span <= a.s.batch) w = pa_seq(a.s, a.nq, a.nk, span - 1);
-  if (row0 >= w.q0 + w.lq) {
-    if (span == 0 || span > a.s.batch) {  // rows of no sequence
-      const int end = (int)min(row0 + S::ROWS, (long)(span == 0 ? pa_clamp(a.s.cu_q[0], a.nq) : a.nq));
-      if (a.dq)
-        for (long i = (row0 * a.dim) + threadIdx.x; i < (long)end * a.dim; i += 256)
-          ((T*)a.dq)[(i / a.dim * a.heads + h) * a.dim + i % a.dim] = (T)0.0f;
-    }
-    if (sums && threadIdx.x < nb) a.part[(slot * a.heads + h) * nb + threadIdx.x] = 0.0f;
-    return;
-  }
-  const int g = h / (a.heads / a.kv_heads);
-  const int i0 = (int)(row0 - w.q0), iw = i0 + wave * 32, i = iw + col;
-  const bool valid = i < w.lq;
-  const int ahead = w.lk - w.lq;
-  int keys = w.lk;
-  if (a.s.causal) keys = min(keys, min(i0 + S::ROWS, w.lq) + ahead);
-
-  Loader<T, DP, S::KEYS, S::WAVES> lk, lv;
-  lk.init((const T*)a.k + (long)w.k0 * a.k_row + g * a.k_head, a.k_row, a.dim);
-  lv.init((const T*)a.v + (long)w.k0 * a.v_row + g * a.v_head, a.v_row, a.dim);
-  const int far = a.s.max_distance;
-  Entry* by_distance = (Entry*)(lds + 2 * S::BUFFER);
-  float* hist = (float*)(by_distance + table_places(far)) + wave * nb * 64;
-  auto load = [&](int n) {
-    char* b = lds + (n & 1) * S::BUFFER;
-    lk.load(b, n * S::KEYS, keys);
-    lv.load(b + Tl::BYTES, n * S::KEYS, keys);
-    if (BIAS && a.s.pos_k) load_words(b + 2 * Tl::BYTES, a.s.pos_k + w.k0, n * S::KEYS, keys);
-  };
-  const int tiles = keys > 0 ? (keys + S::KEYS - 1) / S::KEYS : 0;
-  if (tiles > 0) load(0);
-
-  const long to = ((long)(w.q0 + i) * a.heads + h) * a.dim;
-  frag_t<T> q[Tl::STEPS], dout[Tl::STEPS];
-  load_rows<T>(q, (const T*)a.q + (long)(w.q0 + i) * a.q_row + h * a.q_head, valid, a.dim, half);
-  load_rows<T>(dout, (const T*)a.dout + to, valid, a.dim, half);
-  float delta = 0.0f;
-  if (valid)
-#pragma unroll
-    for (int s = 0; s < Tl::STEPS; ++s) {
-      constexpr int N = 16 / sizeof(T);
-      const int d = (2 * s + half) * N;
-      if (d < a.dim)
-#pragma unroll
-        for (int e = 0; e < N; ++e) delta = fmaf((float)dout[s][e], a.out32_in[to + d + e], delta);
-    }
-  delta += other_half(delta);
-  const long st = (long)h * a.nq + w.q0 + i;
-  const float m = valid ? a.stats[st] : 0.0f, ll = (valid ? a.stats[st + (long)a.heads * a.nq] : INFINITY) - Lift<T>::LOG2;
-  const float ref = m + ll;
-  if (valid && half == 0) a.delta[st] = delta, a.delta[st + (long)a.heads * a.nq] = ref;
-  const float sc = a.scale * PA_LOG2E;
-  const int pos_q = BIAS && valid ? pa_pos_q(a.s, w, i) : 0;
-  if (BIAS) load_table(by_distance, a.s, a.table, h);
-  if (BIAS)
-    for (int c = 0; c < nb; ++c) hist[c * 64 + lane] = 0.0f;
-
-  f32x16 dq[Tl::BLOCKS];
-#pragma unroll
-  for (int b = 0; b < Tl::BLOCKS; ++b) dq[b] = (f32x16)0.0f;
-
-  typename Tl::Lane at(lane);
-  auto tile = [&](auto masked, auto mode, const char* kt, int j0) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(masked)::value;
-    constexpr int MODE = decltype(mode)::value;
-    const char* vt = kt + Tl::BYTES;
-    at.fresh();
-    const int last = a.s.causal ? min(keys, i + ahead + 1) : keys;
-#pragma unroll S::UNROLL
-    for (int kb = 0; kb < S::KEYS / 32; ++kb) {
-      f32x16 x = (f32x16)0.0f, dp = (f32x16)0.0f;
-#pragma unroll
-      for (int s = 0; s < Tl::STEPS; ++s) mma_step(x, Tl::frag(kt, kb * 32, s, at), q[s]);
-      if (S::APART) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < Tl::STEPS; ++s) mma_step(dp, Tl::frag(vt, kb * 32, s, at), dout[s]);
-      if (S::APART) __builtin_amdgcn_sched_barrier(0);
-      Entry e[MODE == NONE ? 1 : 16];
-      float sum = 0.0f;
-      if constexpr (MODE == NONE) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float ds = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -ref)) * (dp[r] - delta);
-          x[r] = MASK && !(j0 + kb * 32 + acc_row(r, half) < last) ? 0.0f : ds;
-        }
-      } else {
-        e[0] = by_distance[j0 < iw + ahead ? 0 : 2 * (far + PAD)];
-        const Entry* near = by_distance + (min(max(j0 + 4 * half - pos_q, -far - 60), far) + far + PAD);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = kb * 32 + acc_row(r, half);
-          if (MODE == ONE) e[r] = e[0];
-          if (MODE == NEAR) e[r] = near[kb * 32 + acc_row(r, 0)];
-          if (MODE == GIVEN) e[r] = by_distance[PAD + pa_entry(pa_apart(((const int*)(vt + Tl::BYTES))[row], pos_q), far)];
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          // hidden by its place or by its bucket: whatever the key and its value hold
-          const float b = MASK && !(j0 + kb * 32 + acc_row(r, half) < last) ? -INFINITY : e[r].bias;
-          const float p = __builtin_amdgcn_exp2f((fmaf(x[r], sc, b) - m) - ll);
-          x[r] = b == -INFINITY ? 0.0f : p * (dp[r] - delta);
-          sum += x[r];
-        }
-      }
-      if (S::APART) __builtin_amdgcn_sched_barrier(0);
-      Probs<T> ds;  // rounded to the type for the product: half a step each, as much as rounding dq once more
-      ds.set(x);
-#pragma unroll
-      for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(kt, kb * 32, b, at, ds, dq[b]);
-      // (behind the products, which run meanwhile)
-      if constexpr (MODE == ONE) {
-        hist[e[0].bucket * 64 + lane] += sum;
-      } else if constexpr (MODE != NONE) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const float four[4] = {x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
-          add_four(hist + lane, e + 4 * t, four);
-        }
-      }
-    }
-  };
-  auto step = [&](int n) {
-    tiles_ready();
-    if (n + 1 < tiles) load(n + 1);
-  };
-  // (counts of tiles; the wave's queries iw .. iw + 31 lie at the keys' places + ahead)
-  Passage way = {};
-  const int whole = keys / S::KEYS;  // tiles with no row behind the last key
-  const int end = iw >= w.lq ? 0 : a.s.causal ? min(tiles, floor_div(iw + 31 + ahead, S::KEYS) + 1) : tiles;
-  way.near0 = way.near1 = way.far1 = max(end, 0);
-  if constexpr (!BIAS) {
-    way.far0 = max(0, min(end, a.s.causal ? min(whole, floor_div(iw + ahead + 1, S::KEYS)) : whole));
-    walk(way, tiles, step, [&](int n) { tile(False(), Mode<NONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); },
-         [&](int n) { tile(True(), Mode<NONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
-  } else if (a.s.pos_q) {
-    walk(way, tiles, step, [](int) {},
-         [&](int n) { tile(True(), Mode<GIVEN>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
-  } else {
-    way.far0 = max(0, min(min(end, whole), floor_div(iw + ahead - far + 1, S::KEYS)));
-    if (!a.s.causal) {
-      way.near0 = max(way.far0, min(end, -floor_div(-(far + iw + 31 + ahead), S::KEYS)));
-      way.far1 = max(way.near0, min(end, whole));
-    }
-    walk(way, tiles, step, [&](int n) { tile(False(), Mode<ONE>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); },
-         [&](int n) { tile(True(), Mode<NEAR>(), lds + (n & 1) * S::BUFFER, n * S::KEYS); });
-  }
-
-  float finite = 0.0f;
-  if (a.dq)
-#pragma unroll
-    for (int b = 0; b < Tl::BLOCKS; ++b)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int d = b * 32 + 8 * t + 4 * half;
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        t4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float z = dq[b][4 * t + e] * (a.scale * Lift<T>::DOWN);
-          finite = fmaf(z, 0.0f, finite);
-          y[e] = (T)z;
-        }
-        if (valid && d < a.dim) *(t4*)((T*)a.dq + to + d) = y;
-      }
-  if (sums) {
-    __syncthreads();
-    const float* all = (const float*)(by_distance + table_places(far));
-    for (int c = wave; c < nb; c += S::WAVES) {
-      float s = 0.0f;
-      for (int v = 0; v < S::WAVES; ++v) s += all[(v * nb + c) * 64 + lane];
-      s = wave_sum(s);
-      if (lane == 0) a.part[(slot * a.heads + h) * nb + c] = s * Lift<T>::DOWN;
-    }
-  }
-  // a hidden pair's 0 times NaN, or a lifted ds beyond fp16: pair by pair
-  const unsigned long long again = __ballot(valid && !(finite == 0.0f));
-  for (unsigned rows = (unsigned)again | (unsigned)(again >> 32); rows; rows &= rows - 1)
-    pa_row_dq<T>(a, w, iw + __ffs(rows) - 1, h);
-}
 
 // The lane's column of a sum, times `factor`, to its row; -> whether any of it is not finite.
 template <typename T, int BLOCKS>
@@ -300,11 +66,12 @@ __global__ __launch_bounds__(256) void pa_dkv_join_kernel(PaArgs a) {
 // RG groups of waves share the keys: each takes its 32 rows of a tile of queries, and their sums are added at the end.  (Four
 // waves with keys of their own are half as many workgroups, each twice as long: 286 us against 222 for eight documents of up
 // to 2048 tokens, 16 heads of 64 over 4.)
-template <typename T, int DP>
+template <typename T, int W>
 struct DkvShape {
   static constexpr int RG = 2;
+  static constexpr int DP = Tile<T, W, 32>::DP;
   static constexpr int WAVES = 4, COLS = 32 * WAVES / RG, ROWS = sizeof(T) == 4 ? 32 * RG : 64, SPAN = ROWS / RG;
-  typedef Tile<T, DP, ROWS> Tl;
+  typedef Tile<T, W, ROWS> Tl;
   static constexpr int BUFFER = 2 * Tl::BYTES + 4 * 256;  // q, dout, delta, stats, positions
   static constexpr int PER_SIMD = DP == 128 ? 1 : 2, UNROLL = DP == 128 || sizeof(T) == 4 ? 1 : 2;
   static constexpr bool APART = DP * sizeof(T) >= 256;
@@ -315,9 +82,9 @@ struct DkvShape {
   }
 };
 
-template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kernel(PaArgs a, long slots) {
-  typedef DkvShape<T, DP> S;
+template <typename T, int W, bool BIAS>
+__global__ __launch_bounds__(256, (DkvShape<T, W>::PER_SIMD)) void pa_dkv_kernel(PaArgs a, long slots) {
+  typedef DkvShape<T, W> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31,
@@ -376,7 +143,7 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
 
   const int h0 = g * group + group * part / a.parts, h1 = g * group + group * (part + 1) / a.parts;
   for (int h = h0; h < h1 && tiles > 0; ++h) {
-    Loader<T, DP, S::ROWS, S::WAVES> lq, ld;
+    Loader<T, W, S::ROWS, S::WAVES> lq, ld;
     lq.init((const T*)a.q + (long)w.q0 * a.q_row + h * a.q_head, a.q_row, a.dim);
     ld.init((const T*)a.dout + ((long)w.q0 * a.heads + h) * a.dim, (long)a.heads * a.dim, a.dim);
     const float* stats = a.stats + (long)h * a.nq + w.q0;
@@ -468,7 +235,7 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
          });
   }
 
-  float* sums = (float*)lds + kg * 2 * 32 * (DP + 4) + col * (DP + 4) + 4 * half;
+  float* sums = (float*)lds + kg * 2 * 32 * (S::DP + 4) + col * (S::DP + 4) + 4 * half;
   __syncthreads();
   if (rg == 1) {
 #pragma unroll
@@ -478,7 +245,7 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
         const f32x4 y = {dk[b][4 * t], dk[b][4 * t + 1], dk[b][4 * t + 2], dk[b][4 * t + 3]};
         const f32x4 z = {dv[b][4 * t], dv[b][4 * t + 1], dv[b][4 * t + 2], dv[b][4 * t + 3]};
         *(f32x4*)(sums + b * 32 + 8 * t) = y;
-        *(f32x4*)(sums + 32 * (DP + 4) + b * 32 + 8 * t) = z;
+        *(f32x4*)(sums + 32 * (S::DP + 4) + b * 32 + 8 * t) = z;
       }
   }
   __syncthreads();
@@ -487,7 +254,7 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
   for (int b = 0; b < Tl::BLOCKS; ++b)
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const f32x4 y = *(const f32x4*)(sums + b * 32 + 8 * t), z = *(const f32x4*)(sums + 32 * (DP + 4) + b * 32 + 8 * t);
+      const f32x4 y = *(const f32x4*)(sums + b * 32 + 8 * t), z = *(const f32x4*)(sums + 32 * (S::DP + 4) + b * 32 + 8 * t);
 #pragma unroll
       for (int e = 0; e < 4; ++e) dk[b][4 * t + e] += y[e], dv[b][4 * t + e] += z[e];
     }
@@ -509,17 +276,18 @@ __global__ __launch_bounds__(256, (DkvShape<T, DP>::PER_SIMD)) void pa_dkv_kerne
 // The same for a head dim of 128, where both gradients' sums and both operands do not leave a SIMD's registers room for a
 // second wave: two waves share the keys, one with k and dv's sums, one with v and dk's.  The first makes the probabilities
 // while the second multiplies dout and v, and hands them over through LDS in fp32.
-template <typename T, int DP>
+template <typename T, int W>
 struct PairShape {
+  static constexpr int DP = Tile<T, W, 32>::DP;
   static constexpr int WAVES = 8, COLS = 128, ROWS = sizeof(T) == 4 ? 32 : 64;
-  typedef Tile<T, DP, ROWS> Tl;
+  typedef Tile<T, W, ROWS> Tl;
   static constexpr int BUFFER = 2 * Tl::BYTES + 4 * 256, PROBS = 4 * ROWS * 32 * 4;
   static int lds(bool bias, int max_distance) { return 2 * BUFFER + PROBS + 64 + (bias ? table_places(max_distance) * 4 : 0); }
 };
 
-template <typename T, int DP, bool BIAS>
+template <typename T, int W, bool BIAS>
 __global__ __launch_bounds__(512, 2) void pa_dkv_pair_kernel(PaArgs a, long slots) {
-  typedef PairShape<T, DP> S;
+  typedef PairShape<T, W> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31,
@@ -578,7 +346,7 @@ __global__ __launch_bounds__(512, 2) void pa_dkv_pair_kernel(PaArgs a, long slot
   typename Tl::Lane at(lane);
   const int h0 = g * group + group * part / a.parts, h1 = g * group + group * (part + 1) / a.parts;
   for (int h = h0; h < h1 && tiles > 0; ++h) {
-    Loader<T, DP, S::ROWS, S::WAVES> lq, ld;
+    Loader<T, W, S::ROWS, S::WAVES> lq, ld;
     lq.init((const T*)a.q + (long)w.q0 * a.q_row + h * a.q_head, a.q_row, a.dim);
     ld.init((const T*)a.dout + ((long)w.q0 * a.heads + h) * a.dim, (long)a.heads * a.dim, a.dim);
     const float* stats = a.stats + (long)h * a.nq + w.q0;
@@ -707,60 +475,46 @@ __global__ __launch_bounds__(512, 2) void pa_dkv_pair_kernel(PaArgs a, long slot
     hipLaunchKernelGGL(KERNEL, dim3(tile_grid(SLOTS, HEADS)), dim3(256), LDS, st, a, SLOTS);               \
   }
 
-template <typename T, int DP>
+template <typename T, int W>
 static bool launch_dkv(const PaArgs& a, hipStream_t st) {
-  typedef DkvShape<T, DP> S;
+  typedef DkvShape<T, W> S;
   const long slots = a.nk / S::COLS + a.s.batch + 2;
   if (a.table)
-    PA_LAUNCH((pa_dkv_kernel<T, DP, true>), slots, a.kv_heads * a.parts, S::lds(true, a.s.max_distance), S::lds(true, PA_MAX_DISTANCE))
-  else PA_LAUNCH((pa_dkv_kernel<T, DP, false>), slots, a.kv_heads * a.parts, S::lds(false, 0), S::lds(false, 0))
+    PA_LAUNCH((pa_dkv_kernel<T, W, true>), slots, a.kv_heads * a.parts, S::lds(true, a.s.max_distance), S::lds(true, PA_MAX_DISTANCE))
+  else PA_LAUNCH((pa_dkv_kernel<T, W, false>), slots, a.kv_heads * a.parts, S::lds(false, 0), S::lds(false, 0))
   return true;
 }
 
-template <typename T, int DP>
+template <typename T, int W>
 static bool launch_pair(const PaArgs& a, hipStream_t st) {
-  typedef PairShape<T, DP> S;
+  typedef PairShape<T, W> S;
   const long slots = a.nk / S::COLS + a.s.batch + 2;
   static bool done[2][64];
 #define PA_PAIR(B)                                                                                                   \
   {                                                                                                                  \
-    if (!i2r_lds_attr((const void*)pa_dkv_pair_kernel<T, DP, B>, S::lds(B, PA_MAX_DISTANCE), done[B])) return false;  \
-    hipLaunchKernelGGL((pa_dkv_pair_kernel<T, DP, B>), dim3(tile_grid(slots, a.kv_heads * a.parts)), dim3(512),       \
+    if (!i2r_lds_attr((const void*)pa_dkv_pair_kernel<T, W, B>, S::lds(B, PA_MAX_DISTANCE), done[B])) return false;  \
+    hipLaunchKernelGGL((pa_dkv_pair_kernel<T, W, B>), dim3(tile_grid(slots, a.kv_heads * a.parts)), dim3(512),       \
                        S::lds(B, a.s.max_distance), st, a, slots);                                                    \
   }
   if (a.table) PA_PAIR(true) else PA_PAIR(false)
   return true;
 }
 
-template <typename T, int DP>
-static bool launch_bwd(const PaArgs& a, hipStream_t st, bool dq, bool dkv) {
-  const int far = a.s.max_distance;
-  const long slots_q = (a.nq >> 7) + a.s.batch + 2;
-  if (dq) {
-    typedef DqShape<T, DP> S;
-    if (a.table) PA_LAUNCH((pa_dq_kernel<T, DP, true>), slots_q, a.heads, S::lds(true, far, a.s.num_buckets),
-                           S::lds(true, PA_MAX_DISTANCE, PA_MAX_BUCKETS))
-    else PA_LAUNCH((pa_dq_kernel<T, DP, false>), slots_q, a.heads, S::lds(false, 0, 0), S::lds(false, 0, 0))
-  }
-  if (dkv) {
-    bool ok;
-    // 128 wide: one wave a SIMD against the pair's two; four documents of 2048 tokens, 32 heads: bf16 1126 us against 938, but
-    // fp32, whose products take 8 times as long and hide everything else, 1403 against 1487 (1024 tokens)
-    if constexpr (DP == 128 && sizeof(T) == 2) ok = launch_pair<T, DP>(a, st);
-    else ok = launch_dkv<T, DP>(a, st);
-    if (!ok) return false;
-    if (a.parts > 1)
-      hipLaunchKernelGGL(pa_dkv_join_kernel<T>, dim3(i2r_cdiv((long)a.nk * a.kv_heads, 4)), dim3(256), 0, st, a);
-  }
-  return true;
+template <typename T, int W>
+static bool launch_both(const PaArgs& a, hipStream_t st) {
+  bool ok;
+  // 128 wide: one wave a SIMD against the pair's two; eight documents of 2048 tokens, 32 heads: bf16 1126 us against 938, but
+  // fp32, whose products take 8 times as long and hide everything else, 1403 against 1487 (1024 tokens)
+  if constexpr (W > 64 && sizeof(T) == 2) ok = launch_pair<T, W>(a, st);
+  else ok = launch_dkv<T, W>(a, st);
+  if (ok && a.parts > 1)
+    hipLaunchKernelGGL(pa_dkv_join_kernel<T>, dim3(i2r_cdiv((long)a.nk * a.kv_heads, 4)), dim3(256), 0, st, a);
+  return ok;
 }
 
-bool pa_launch_bwd(int dtype, const PaArgs& a, hipStream_t st, bool dq, bool dkv) {
-#define PA_BY_DIM(T)                                            \
-  return a.dim <= 32   ? launch_bwd<T, 32>(a, st, dq, dkv)      \
-         : a.dim <= 64 ? launch_bwd<T, 64>(a, st, dq, dkv)      \
-                       : launch_bwd<T, 128>(a, st, dq, dkv);
-  if (dtype == 0) PA_BY_DIM(float)
-  if (dtype == 1) PA_BY_DIM(f16_t)
-  PA_BY_DIM(bf16_t)
+bool pa_launch_dkv(int dtype, const PaArgs& a, hipStream_t st) {
+#define PA_CALL(T, W) launch_both<T, W>(a, st)
+  if (dtype == 0) PA_BY_WIDTH(float, PA_CALL);
+  if (dtype == 1) PA_BY_WIDTH(f16_t, PA_CALL);
+  PA_BY_WIDTH(bf16_t, PA_CALL);
 }

@@ -3,17 +3,18 @@
 
 // One workgroup: 4 waves x 32 queries of one sequence and head; keys come in tiles of KEYS, the next tile loading while
 // this one is worked on (two LDS buffers, one barrier a tile).
-template <typename T, int DP>
+template <typename T, int W>
 struct FwdShape {
+  static constexpr int DP = Tile<T, W, 32>::DP;
   static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
-  typedef Tile<T, DP, KEYS> Tl;
+  typedef Tile<T, W, KEYS> Tl;
   static constexpr int BUFFER = 2 * Tl::BYTES + 256;  // k, v, positions
   static int lds(bool bias, int max_distance) { return 2 * BUFFER + (bias ? table_places(max_distance) * 4 : 0); }
 };
 
-template <typename T, int DP, bool BIAS, bool SAVE>
+template <typename T, int W, bool BIAS, bool SAVE>
 __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
-  typedef FwdShape<T, DP> S;
+  typedef FwdShape<T, W> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31,
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
   int keys = w.lk;                // keys that the workgroup's last query sees
   if (a.s.causal) keys = min(keys, min(i0 + S::ROWS, w.lq) + ahead);
 
-  Loader<T, DP, S::KEYS, S::WAVES> lk, lv;
+  Loader<T, W, S::KEYS, S::WAVES> lk, lv;
   lk.init((const T*)a.k + (long)w.k0 * a.k_row + g * a.k_head, a.k_row, a.dim);
   lv.init((const T*)a.v + (long)w.k0 * a.v_row + g * a.v_head, a.v_row, a.dim);
   float* by_distance = (float*)(lds + 2 * S::BUFFER);
@@ -203,9 +204,9 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
     pa_row_fwd<T>(a, w, iw + __ffs(rows) - 1, h);
 }
 
-template <typename T, int DP>
-static void launch_fwd(const PaArgs& a, hipStream_t st, bool& ok) {
-  typedef FwdShape<T, DP> S;
+template <typename T, int W>
+static bool launch_fwd(const PaArgs& a, hipStream_t st) {
+  typedef FwdShape<T, W> S;
   const bool bias = a.table != nullptr, save = a.stats != nullptr;
   const long slots = (a.nq >> 7) + a.s.batch + 2;
   const int lds = S::lds(bias, a.s.max_distance);
@@ -213,24 +214,19 @@ static void launch_fwd(const PaArgs& a, hipStream_t st, bool& ok) {
 #define PA_FWD(B, V)                                                                                \
   {                                                                                                 \
     static bool done[64];                                                                           \
-    ok = i2r_lds_attr((const void*)pa_fwd_kernel<T, DP, B, V>, S::lds(true, PA_MAX_DISTANCE), done); \
-    if (ok) hipLaunchKernelGGL((pa_fwd_kernel<T, DP, B, V>), grid, dim3(256), lds, st, a, slots);   \
+    if (!i2r_lds_attr((const void*)pa_fwd_kernel<T, W, B, V>, S::lds(true, PA_MAX_DISTANCE), done)) return false; \
+    hipLaunchKernelGGL((pa_fwd_kernel<T, W, B, V>), grid, dim3(256), lds, st, a, slots);   \
   }
   if (bias && save) PA_FWD(true, true)
   else if (bias) PA_FWD(true, false)
   else if (save) PA_FWD(false, true)
   else PA_FWD(false, false)
+  return true;
 }
 
 bool pa_launch_fwd(int dtype, const PaArgs& a, hipStream_t st) {
-  bool ok = true;
-  const int dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
-#define PA_BY_DIM(T)                          \
-  if (dp == 32) launch_fwd<T, 32>(a, st, ok); \
-  else if (dp == 64) launch_fwd<T, 64>(a, st, ok); \
-  else launch_fwd<T, 128>(a, st, ok);
-  if (dtype == 0) { PA_BY_DIM(float) }
-  else if (dtype == 1) { PA_BY_DIM(f16_t) }
-  else { PA_BY_DIM(bf16_t) }
-  return ok;
+#define PA_CALL(T, W) launch_fwd<T, W>(a, st)
+  if (dtype == 0) PA_BY_WIDTH(float, PA_CALL);
+  if (dtype == 1) PA_BY_WIDTH(f16_t, PA_CALL);
+  PA_BY_WIDTH(bf16_t, PA_CALL);
 }

@@ -39,13 +39,23 @@ __device__ __forceinline__ void mma_step(f32x16& c, frag_t<float> a, frag_t<floa
   for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
 }
 
+// Head dims are worked on in five widths W: one step of a product (32 bytes: 8 fp32 or 16 elements of 16 bits), 32, 64, 96 and
+// 128; rows lie in LDS in 32, 64 or 128 elements.
+#define PA_BY_WIDTH(T, CALL)                                                       \
+  return a.dim <= 32 / (int)sizeof(T) ? CALL(T, 32 / (int)sizeof(T))               \
+         : a.dim <= 32 ? CALL(T, 32)                                               \
+         : a.dim <= 64 ? CALL(T, 64)                                               \
+         : a.dim <= 96 ? CALL(T, 96)                                               \
+                       : CALL(T, 128)
+
 // A tile of ROWS rows of DP elements (the head dim padded with zeros), 16-byte chunks of a row exchanged by its number so
 // that the 32 rows of a fragment read, and the 4 x 64 bytes of a transposed one, fall on different banks.
-template <typename T, int DP, int ROWS>
+template <typename T, int W, int ROWS>
 struct Tile {
+  static constexpr int DP = W <= 32 ? 32 : W <= 64 ? 64 : 128;
   static constexpr int ROW_BYTES = DP * (int)sizeof(T), CHUNKS = ROW_BYTES / 16, BYTES = ROWS * ROW_BYTES;
-  static constexpr int STEPS = ROW_BYTES / 32;  // steps of a product over the head dim
-  static constexpr int BLOCKS = DP / 32;        // 32-wide blocks of the head dim
+  static constexpr int STEPS = W * (int)sizeof(T) / 32;  // steps of a product over the head dim
+  static constexpr int BLOCKS = (W + 31) / 32;           // 32-wide blocks of the head dim
 
   // (made of the row's bits by exclusive or: what two disjoint sets of bits give is the exclusive or of both)
   __host__ __device__ static constexpr int swizzle(int row) {
@@ -128,9 +138,9 @@ struct Probs<float> {
 // Loads tiles of rows of one (sequence, head) into LDS without passing through registers, by WAVES waves together or (1)
 // by each wave for itself.  Rows behind the last and
 // columns behind the head dim are out of the descriptor's range and arrive as zeros.
-template <typename T, int DP, int ROWS, int WAVES>
+template <typename T, int W, int ROWS, int WAVES>
 struct Loader {
-  typedef Tile<T, DP, ROWS> Tl;
+  typedef Tile<T, W, ROWS> Tl;
   static constexpr int LOADS = Tl::BYTES / (1024 * WAVES);  // 1 KiB for each wave and instruction
   static_assert(LOADS * 1024 * WAVES == Tl::BYTES, "a tile has to be whole instructions of all waves");
   const char* base;

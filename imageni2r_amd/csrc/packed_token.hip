@@ -5,12 +5,13 @@
 // its own tiles and no barrier), whose parts a second kernel joins in a fixed order.
 #include "packed_tiles.h"
 
-template <typename T, int DP>
+template <typename T, int W>
 struct TokenShape {
+  static constexpr int DP = Tile<T, W, 32>::DP;
   static constexpr int KEYS = 32, STAGE = 2 * KEYS * DP * (int)sizeof(T);  // k and v of 32 keys
   // 64 KiB of tiles a workgroup (two of them on a CU): as many waves as that feeds with two stages each
   static constexpr int WAVES = 65536 / (2 * STAGE) < 4 ? 65536 / (2 * STAGE) : 4;
-  typedef Tile<T, DP, KEYS> Tl;
+  typedef Tile<T, W, KEYS> Tl;
   static constexpr int PER_WAVE = 2 * STAGE, PER_SIMD = WAVES == 1 ? 1 : 2;
   static_assert(32 * (DP + 4) * 4 <= PER_WAVE, "a wave's sums go where its tiles were");
   static constexpr int SMALL = WAVES * 32 * 8 + 32 * 4;  // m and l of the waves, marks
@@ -24,9 +25,9 @@ struct TokenPlan {
   float *o, *ml;                     // parts: (split, row, head, dim) and (split, {m, l}, row, head)
 };
 
-template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>::PER_SIMD)) void pa_token_kernel(PaArgs a, TokenPlan p) {
-  typedef TokenShape<T, DP> S;
+template <typename T, int W, bool BIAS>
+__global__ __launch_bounds__((64 * TokenShape<T, W>::WAVES), (TokenShape<T, W>::PER_SIMD)) void pa_token_kernel(PaArgs a, TokenPlan p) {
+  typedef TokenShape<T, W> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
@@ -64,10 +65,10 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>
 
   char* tiles = lds + wave * S::PER_WAVE;
   float* small = (float*)(lds + S::WAVES * S::PER_WAVE);
-  Loader<T, DP, 32, 1> lk, lv;
+  Loader<T, W, 32, 1> lk, lv;
   lk.init((const T*)a.k + (long)w.k0 * a.k_row + g * a.k_head, a.k_row, a.dim);
   lv.init((const T*)a.v + (long)w.k0 * a.v_row + g * a.v_head, a.v_row, a.dim);
-  constexpr int LOADS = 2 * Loader<T, DP, 32, 1>::LOADS;
+  constexpr int LOADS = 2 * Loader<T, W, 32, 1>::LOADS;
   auto load = [&](int n, int b) {
     char* t = tiles + (n & 1) * S::STAGE;
     asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // what was there has been read
@@ -195,7 +196,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>
       f32x4 z;
 #pragma unroll
       for (int c = 0; c < 4; ++c) z[c] = o[t][4 * e + c] * fall;
-      *(f32x4*)(mine + col * (DP + 4) + t * 32 + 8 * e + 4 * half) = z;
+      *(f32x4*)(mine + col * (S::DP + 4) + t * 32 + 8 * e + 4 * half) = z;
     }
   // (the sums of another column than the thread's own are needed below)
   __syncthreads();
@@ -208,7 +209,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP>::WAVES), (TokenShape<T, DP>
     if (t >= 1 << p.shift || hh >= group || i0 + t >= w.lq) continue;
     f32x4 z = (f32x4)0.0f;
 #pragma unroll
-    for (int v = 0; v < S::WAVES; ++v) z += *(const f32x4*)((const float*)(lds + v * S::PER_WAVE) + c * (DP + 4) + d);
+    for (int v = 0; v < S::WAVES; ++v) z += *(const f32x4*)((const float*)(lds + v * S::PER_WAVE) + c * (S::DP + 4) + d);
     const long rh = (long)(w.q0 + i0 + t) * a.heads + g * group + hh;
     if (p.splits > 1) {
       if (wm[c] != -INFINITY) *(f32x4*)(p.o + (split * parts + rh) * a.dim + d) = z;
@@ -351,18 +352,18 @@ long pa_token_ws_bytes(int batch, int nq, int nk, int heads, int kv_heads, int d
   return p.splits > 1 ? (long)p.splits * nq * heads * (dim + 2) * 4 : 0;
 }
 
-template <typename T, int DP>
+template <typename T, int W>
 static bool launch_token(const PaArgs& a, const TokenPlan& p, hipStream_t st) {
-  typedef TokenShape<T, DP> S;
+  typedef TokenShape<T, W> S;
   const long slots = (a.nq >> p.shift) + a.s.batch + 2;
   const dim3 grid((unsigned)(slots * a.kv_heads * p.chunks * p.splits));
   static bool done[2][64];
   if (a.table) {
-    if (!i2r_lds_attr((const void*)pa_token_kernel<T, DP, true>, S::lds(true, PA_MAX_DISTANCE), done[1])) return false;
-    hipLaunchKernelGGL((pa_token_kernel<T, DP, true>), grid, dim3(64 * S::WAVES), S::lds(true, a.s.max_distance), st, a, p);
+    if (!i2r_lds_attr((const void*)pa_token_kernel<T, W, true>, S::lds(true, PA_MAX_DISTANCE), done[1])) return false;
+    hipLaunchKernelGGL((pa_token_kernel<T, W, true>), grid, dim3(64 * S::WAVES), S::lds(true, a.s.max_distance), st, a, p);
   } else {
-    if (!i2r_lds_attr((const void*)pa_token_kernel<T, DP, false>, S::lds(false, 0), done[0])) return false;
-    hipLaunchKernelGGL((pa_token_kernel<T, DP, false>), grid, dim3(64 * S::WAVES), S::lds(false, 0), st, a, p);
+    if (!i2r_lds_attr((const void*)pa_token_kernel<T, W, false>, S::lds(false, 0), done[0])) return false;
+    hipLaunchKernelGGL((pa_token_kernel<T, W, false>), grid, dim3(64 * S::WAVES), S::lds(false, 0), st, a, p);
   }
   if (p.splits > 1) {
     const int threads = std::min(1024, (std::min(p.splits, 128) * (a.dim / 4) + 63) / 64 * 64);
@@ -375,9 +376,8 @@ bool pa_launch_token(int dtype, const PaArgs& a, void* ws, hipStream_t st) {
   TokenPlan p = token_plan(a.s.batch, a.nq, a.nk, a.heads, a.kv_heads);
   p.o = (float*)ws;
   p.ml = p.o + (long)p.splits * a.nq * a.heads * a.dim;
-#define PA_BY_DIM(T) \
-  return a.dim <= 32 ? launch_token<T, 32>(a, p, st) : a.dim <= 64 ? launch_token<T, 64>(a, p, st) : launch_token<T, 128>(a, p, st);
-  if (dtype == 0) PA_BY_DIM(float)
-  if (dtype == 1) PA_BY_DIM(f16_t)
-  PA_BY_DIM(bf16_t)
+#define PA_CALL(T, W) launch_token<T, W>(a, p, st)
+  if (dtype == 0) PA_BY_WIDTH(float, PA_CALL);
+  if (dtype == 1) PA_BY_WIDTH(f16_t, PA_CALL);
+  PA_BY_WIDTH(bf16_t, PA_CALL);
 }
