@@ -102,8 +102,9 @@ class PackedSequences:
     ``pos_q``), or without them by j and i + Lk - Lq.
 
     All arrays are int32 vectors on the HIP device, read by the kernels when they run: an object stays valid when their
-    values change (a cache that grows, a replayed graph).  Nothing checks the values on the host; the kernels clamp them
-    to the tensors they are used with, and sequences have to ascend."""
+    values change (a cache that grows, a replayed graph) -- between a forward and its backward they must not.  Nothing
+    checks the values on the host: the kernels clamp them to the tensors they are used with, and sequences have to
+    ascend."""
 
     def __init__(self, cu_q, cu_k=None, *, len_k=None, causal=False, buckets=None, pos_q=None, pos_k=None):
         _index(cu_q, "cu_q")
@@ -138,6 +139,25 @@ class PackedSequences:
         return cls(torch.tensor(cu, dtype=torch.int32, device=device), **kw)
 
 
+    @classmethod
+    def of_observed(cls, mask, buckets=None):
+        """For series whose every step asks but whose observed steps alone answer: ``mask`` (B, L) bool, True where a step
+        was observed.  -> (sequences, order): queries are all B * L rows, keys the rows ``order`` of them, of which those
+        of a series lie together (rows of ``order`` behind the last series' are no keys).  With ``buckets`` positions are
+        the steps.  Nothing waits for the device."""
+        if mask.dtype != torch.bool or mask.dim() != 2:
+            raise TypeError(f"mask: expected a (B, L) bool tensor, got {tuple(mask.shape)} {mask.dtype}")
+        B, L = mask.shape
+        dev = mask.device
+        cu_q = torch.arange(0, (B + 1) * L, L, dtype=torch.int32, device=dev)
+        cu_k = torch.zeros(B + 1, dtype=torch.int32, device=dev)
+        torch.cumsum(mask.sum(1, dtype=torch.int32), 0, out=cu_k[1:])
+        order = (~mask).reshape(-1).to(torch.uint8).argsort(stable=True)
+        pos = dict(pos_q=torch.arange(L, dtype=torch.int32, device=dev).repeat(B),
+                   pos_k=(order % L).to(torch.int32)) if buckets is not None else {}
+        return cls(cu_q, cu_k, buckets=buckets, **pos), order
+
+
 def _rows(t, name, dtype, device):
     """A (rows, heads, dim) operand: in place where its rows are contiguous and 16-byte aligned, else a copy."""
     if t.dim() != 3:
@@ -147,7 +167,8 @@ def _rows(t, name, dtype, device):
     if t.device != device:
         raise ValueError(f"{name}: on {t.device}, the sequences on {device}")
     s0, s1, s2 = t.stride()
-    if s2 != 1 or (s0 * t.element_size()) % 16 or (s1 * t.element_size()) % 16 or t.data_ptr() % 16 or max(s0, s1) >= 1 << 22:
+    whole = 4 if dtype is torch.float32 else 8
+    if s2 != 1 or (s0 | s1) % whole or t.data_ptr() % 16 or s0 >= 1 << 22 or s1 >= 1 << 22:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -192,17 +213,35 @@ def _check(q, k, v, seqs, bias):
     return q, k, v
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call(device, name, *args):
     """The call on ``device``'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, ops._stream())
+    index = device.index
+    if index == _current_device():
+        _lib.call(name, *args, ops._stream() if _raw_stream is None else _raw_stream(index))
     else:
         with torch.cuda.device(device):
             _lib.call(name, *args, ops._stream())
 
 
-def _workspace(n, device):
-    return torch.empty((n,), dtype=torch.uint8, device=device) if n > 0 else None
+_sizes = {}
+
+
+def _workspace(device, name, *sizes):
+    """-> (workspace or None, its address or None, its bytes) of an entry point for these sizes."""
+    key = (name,) + sizes
+    n = _sizes.get(key)
+    if n is None:
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        n = _sizes[key] = _lib.query(name, *sizes)
+    if n <= 0:
+        return None, None, 0
+    ws = torch.empty((n,), dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), n
 
 
 def packed_attention_fwd(q, k, v, seqs, bias=None, scale=None, out=None, save=False):
@@ -221,11 +260,10 @@ def packed_attention_fwd(q, k, v, seqs, bias=None, scale=None, out=None, save=Fa
     if save:
         out32 = out if dt == 0 else torch.empty((nq, heads, dim), dtype=torch.float32, device=dev)
         stats = torch.empty((2, heads, nq), dtype=torch.float32, device=dev)
-    n = _lib.query("i2r_packed_attention_fwd_ws_bytes", dt, seqs.batch, nq, nk, heads, kv_heads, dim)
-    ws = _workspace(n, dev)
+    ws, at, n = _workspace(dev, "i2r_packed_attention_fwd_ws_bytes", dt, seqs.batch, nq, nk, heads, kv_heads, dim)
     _call(dev, "i2r_packed_attention_fwd", seqs._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           None if bias is None else bias.data_ptr(), out.data_ptr(), None if dt == 0 or not save else out32.data_ptr(),
-          None if stats is None else stats.data_ptr(), None if ws is None else ws.data_ptr(), n, dt, nq, nk, heads,
+          None if stats is None else stats.data_ptr(), at, n, dt, nq, nk, heads,
           kv_heads, dim, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
           float(dim**-0.5 if scale is None else scale), int(fresh))
     return out, out32, stats
@@ -253,11 +291,10 @@ def packed_attention_bwd(q, k, v, seqs, bias, out32, stats, dout, scale=None, ne
     dk = torch.empty((nk, kv_heads, dim), dtype=q.dtype, device=dev) if need_dkv else None
     dv = torch.empty_like(dk) if need_dkv else None
     dbias = torch.empty((heads, nb), dtype=torch.float32, device=dev) if need_dbias else None
-    n = _lib.query("i2r_packed_attention_bwd_ws_bytes", dt, seqs.batch, nq, nk, heads, kv_heads, dim, nb)
-    ws = _workspace(n, dev)
+    ws, at, n = _workspace(dev, "i2r_packed_attention_bwd_ws_bytes", dt, seqs.batch, nq, nk, heads, kv_heads, dim, nb)
     _call(dev, "i2r_packed_attention_bwd", seqs._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           None if bias is None else bias.data_ptr(), out32.data_ptr(), stats.data_ptr(), dout.data_ptr(),
-          *(None if t is None else t.data_ptr() for t in (dq, dk, dv, dbias, ws)), n, dt, nq, nk, heads, kv_heads, dim,
+          *(None if t is None else t.data_ptr() for t in (dq, dk, dv, dbias)), at, n, dt, nq, nk, heads, kv_heads, dim,
           q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
           float(dim**-0.5 if scale is None else scale))
     return dq, dk, dv, dbias
@@ -331,10 +368,9 @@ def relative_bias_bwd(dout, buckets, pos_q=None, pos_k=None):
     heads, q_len, k_len = dout.shape
     dtable = torch.empty((heads, buckets.num_buckets), dtype=torch.float32, device=dout.device)
     _check_bias(dtable, buckets, q_len, k_len, pos_q, pos_k, dout.dtype)
-    n = _lib.query("i2r_relative_bias_bwd_ws_bytes", heads, q_len, k_len, buckets.num_buckets)
-    ws = _workspace(n, dout.device)
+    ws, at, n = _workspace(dout.device, "i2r_relative_bias_bwd_ws_bytes", heads, q_len, k_len, buckets.num_buckets)
     _call(dout.device, "i2r_relative_bias_bwd", dout.data_ptr(), buckets.on(dout.device).data_ptr(), ops._p(pos_q),
-          ops._p(pos_k), dtable.data_ptr(), ops._p(ws), n, _DTYPES[dout.dtype], heads, q_len, k_len, buckets.num_buckets,
+          ops._p(pos_k), dtable.data_ptr(), at, n, _DTYPES[dout.dtype], heads, q_len, k_len, buckets.num_buckets,
           buckets.max_distance)
     return dtable
 

@@ -21,6 +21,10 @@ the SAME iteration without the three things that cost time and change no trained
   backward).  Exact when the TST is deterministic; with its dropout live the two passes differ only in their masks;
 * no ``empty_cache()``: the caching allocator keeps its blocks (the replayed diffusion graph owns its memory anyway).
 
+With ``packed`` the stand-in's encoder layers attend on the HIP path (imageni2r_amd.packed): the observed steps' keys and
+values lie packed, missing steps cost no scores, and a series without any observed step comes out finite; ``rel_buckets``
+adds a learned bias by the distance in time.
+
 ``TrainIteration`` is the drop-in loop body; ``CompletionStandIn`` is a builder-written torch.nn network with the TST
 stage's shapes (d_model 40, 5 heads, 6 layers, feed-forward 2048, 3-layer bi-GRU decoder: utils/utils_args.py:65-82,
 run_irregular.py:143-163) used by tools/tst_boundary_bench.py and the tests -- it is NOT the reference's model and
@@ -33,14 +37,26 @@ import math
 import torch
 import torch.nn as nn
 
+from .packed import PackedSequences, RelativeBuckets, packed_attention
+
 
 class CompletionStandIn(nn.Module):
     """Transformer encoder over (B, L, C) with a key-padding mask + 3-layer bidirectional GRU decoder + sigmoid:
     the layer types and sizes of the reference's completion stage, written from its configuration (see module doc)."""
 
-    def __init__(self, feat_dim, max_len, d_model=40, n_heads=5, num_layers=6, dim_feedforward=2048, dropout=0.1):
+    def __init__(self, feat_dim, max_len, d_model=40, n_heads=5, num_layers=6, dim_feedforward=2048, dropout=0.1,
+                 packed=False, rel_buckets=0, rel_distance=128):
+        """``packed``: attention by packed_attention, with the same parameters and, without a bias, the same values; the
+        attention probabilities are not dropped out.  ``rel_buckets`` > 0 (with ``packed``): one learned bias table
+        (n_heads, rel_buckets) for all layers, zero at first."""
         super().__init__()
+        if rel_buckets and not packed:
+            raise ValueError("rel_buckets needs packed=True")
         self.d_model = d_model
+        self.n_heads, self.packed = n_heads, bool(packed)
+        self.buckets = RelativeBuckets(rel_buckets, rel_distance) if rel_buckets else None
+        if rel_buckets:
+            self.rel_bias = nn.Parameter(torch.zeros(n_heads, rel_buckets))
         self.project_inp = nn.Linear(feat_dim, d_model)
         pos = torch.arange(max_len, dtype=torch.float32)[:, None]
         div = torch.exp(torch.arange(0, d_model, 2, dtype=torch.float32) * (-math.log(10000.0) / d_model))
@@ -59,8 +75,23 @@ class CompletionStandIn(nn.Module):
     def embed(self, x, padding_masks):
         z = torch.nan_to_num(x, nan=0.0)
         z = self.drop(self.project_inp(z) * math.sqrt(self.d_model) + self.pe[:, : z.shape[1]])
-        z = self.encoder(z, src_key_padding_mask=~padding_masks)
+        z = self._encode_packed(z, padding_masks) if self.packed else self.encoder(z, src_key_padding_mask=~padding_masks)
         return self.output_layer(self.drop(torch.nn.functional.gelu(z)))
+
+    def _encode_packed(self, z, padding_masks):
+        """The encoder with each series' keys and values packed to its observed steps."""
+        B, L, _ = z.shape
+        F = torch.nn.functional
+        seqs, order = PackedSequences.of_observed(padding_masks, self.buckets)
+        bias = self.rel_bias if self.buckets is not None else None
+        z = z.reshape(B * L, self.d_model)
+        for layer in self.encoder.layers:
+            a = layer.self_attn
+            qkv = F.linear(z, a.in_proj_weight, a.in_proj_bias).view(B * L, 3, self.n_heads, -1)
+            h = packed_attention(qkv[:, 0], qkv[order, 1], qkv[order, 2], seqs, bias=bias)
+            z = layer.norm1(z + layer.dropout1(a.out_proj(h.reshape(B * L, self.d_model))))
+            z = layer.norm2(z + layer.dropout2(layer.linear2(layer.dropout(layer.activation(layer.linear1(z))))))
+        return z.view(B, L, self.d_model)
 
     def decode(self, h):
         out, _ = self.rnn(h)
