@@ -8,12 +8,13 @@ struct FwdShape {
   static constexpr int DP = Tile<T, W, 32>::DP;
   static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
   typedef Tile<T, W, KEYS> Tl;
+  static constexpr int MOST = W > 64 ? 2 : 4;
   static constexpr int BUFFER = 2 * Tl::BYTES + 256;  // k, v, positions
   static int lds(bool bias, int max_distance) { return 2 * BUFFER + (bias ? table_places(max_distance) * 4 : 0); }
 };
 
 template <typename T, int W, bool BIAS, bool SAVE>
-__global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
+__global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, FwdShape<T, W>::MOST))) void pa_fwd_kernel(PaArgs a, long slots) {
   typedef FwdShape<T, W> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
@@ -81,10 +82,18 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
     at.fresh();
     f32x16 x[BLOCKS];
 #pragma unroll
-    for (int kb = 0; kb < BLOCKS; ++kb) {
-      x[kb] = (f32x16)0.0f;
+    for (int kb = 0; kb < BLOCKS; ++kb) x[kb] = (f32x16)0.0f;
 #pragma unroll
-      for (int s = 0; s < Tl::STEPS; ++s) mma_step(x[kb], Tl::frag(kt, kb * 32, s, at), q[s]);
+    for (int s = 0; s < Tl::STEPS; ++s)
+#pragma unroll
+      for (int kb = 0; kb < BLOCKS; ++kb) mma_step(x[kb], Tl::frag(kt, kb * 32, s, at), q[s]);
+    // v's operands of the first 32 keys set out before the softmax, which hides their way
+    constexpr bool EARLY = sizeof(T) == 2 && !(BIAS && SAVE);
+    typename Tl::Turned early[EARLY ? Tl::BLOCKS : 1];
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int b = 0; b < Tl::BLOCKS; ++b) early[b] = Tl::turned(vt, 0, b, at);
+      __builtin_amdgcn_sched_barrier(0);
     }
     const float one = MODE == ONE ? by_distance[j0 < iw + ahead ? 0 : 2 * (far + PAD)] : 0.0f;
     // the place of the tile's first row (clamped so far out that all rows' places are beyond max_distance)
@@ -140,7 +149,14 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(PaArgs a, long slots) {
       } else {
         p.set(x[kb]);
 #pragma unroll
-        for (int b = 0; b < Tl::BLOCKS; ++b) Tl::mma_t(vt, kb * 32, b, at, p, o[b]);
+        for (int b = 0; b < Tl::BLOCKS; ++b) {
+          if constexpr (EARLY) {
+            if (kb == 0) Tl::mma_turned(early[b], p, o[b]);
+            else Tl::mma_t(vt, kb * 32, b, at, p, o[b]);
+          } else {
+            Tl::mma_t(vt, kb * 32, b, at, p, o[b]);
+          }
+        }
       }
     }
   };

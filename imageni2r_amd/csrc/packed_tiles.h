@@ -57,9 +57,14 @@ struct Tile {
   static constexpr int STEPS = W * (int)sizeof(T) / 32;  // steps of a product over the head dim
   static constexpr int BLOCKS = (W + 31) / 32;           // 32-wide blocks of the head dim
 
-  // (made of the row's bits by exclusive or: what two disjoint sets of bits give is the exclusive or of both)
+  // What a row's chunk numbers are exchanged by (exclusive or).  LDS has 64 banks of 4 bytes: of 16 rows' equal chunks, and of
+  // the 4 x 64 bytes (fp32: 2 x 128) of a transposed read, each has to fall on 16 bytes, of 256, of its own.  Made of the
+  // row's bits, so that what two disjoint sets of bits give is the exclusive or of both.
   __host__ __device__ static constexpr int swizzle(int row) {
-    return CHUNKS >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : CHUNKS == 8 ? ((row & 1) << 2) | ((row >> 1) & 3) : (row >> 1) & 3;
+    return CHUNKS >= 16 ? (sizeof(T) == 2 ? ((row & 3) << 2) | ((row >> 2) & 3)
+                                          : ((row & 4) << 1) | ((row & 3) << 1) | ((row >> 3) & 1))
+           : CHUNKS == 8 ? ((row & 2) << 1) | ((row >> 2) & 3)
+                         : (row >> 2) & 3;
   }
 
   // A lane's two places in a block of 32 rows, from which every other differs by constants.  fresh() keeps the compiler
@@ -84,6 +89,34 @@ struct Tile {
     return *(const frag_t<T>*)(tile + r0 * ROW_BYTES + (at.f ^ (s << 5)));
   }
 
+  // Transposed operands of rows r0 .. r0 + 32, 32 d of block db (16-bit types)
+  struct Turned {
+    s16x4 part[2][2];
+  };
+  __device__ static __forceinline__ Turned turned(const char* tile, int r0, int db, const Lane& at) {
+    // ds_read_b64_tr_b16: of each 16 lanes, lane n addresses 4 elements of row n >> 2, and gets column n of the 4 rows
+    Turned x;
+    const unsigned base = (unsigned)(uintptr_t)tile;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = 16 * c + 8 * e;
+        typedef __attribute__((address_space(3))) char lds_char;
+        lds_char* from = (lds_char*)(base + (at.t ^ (db << 6) ^ (swizzle(row) << 4))) + (r0 + row) * ROW_BYTES;
+        x.part[c][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from);
+      }
+    return x;
+  }
+  template <typename P>
+  __device__ static __forceinline__ void mma_turned(const Turned& x, const P& p, f32x16& acc) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const s16x8 a = __builtin_shufflevector(x.part[c][0], x.part[c][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      mma_step(acc, __builtin_bit_cast(frag_t<T>, a), p[c]);
+    }
+  }
+
   // acc[32 d of block db][columns] += tile(rows r0 .. r0 + 32)^T p, p the accumulators of those rows
   template <typename P>
   __device__ static __forceinline__ void mma_t(const char* tile, int r0, int db, const Lane& at, const P& p, f32x16& acc) {
@@ -95,19 +128,7 @@ struct Tile {
         acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc, 0, 0, 0);
       }
     } else {
-      // ds_read_b64_tr_b16: of each 16 lanes, lane n addresses 4 elements of row n >> 2, and gets column n of the 4 rows
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        s16x4 part[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = 16 * c + 8 * e;
-          part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              LDS_PTR(s16x4, (char*)tile + (r0 + row) * ROW_BYTES + (at.t ^ (db << 6) ^ (swizzle(row) << 4))));
-        }
-        const s16x8 a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        mma_step(acc, __builtin_bit_cast(frag_t<T>, a), p[c]);
-      }
+      mma_turned(turned(tile, r0, db, at), p, acc);
     }
   }
 };
