@@ -379,11 +379,11 @@ __global__ __launch_bounds__(512, 2) void pa_dkv_pair_kernel(PaArgs a, long slot
       f32x16 x[PARTS];
       const char* left = second ? dt : qt;
 #pragma unroll
-      for (int qb = 0; qb < PARTS; ++qb) {
-        x[qb] = (f32x16)0.0f;
+      for (int qb = 0; qb < PARTS; ++qb) x[qb] = (f32x16)0.0f;
 #pragma unroll
-        for (int s = 0; s < Tl::STEPS; ++s) mma_step(x[qb], Tl::frag(left, qb * 32, s, at), kv[s]);
-      }
+      for (int s = 0; s < Tl::STEPS; ++s)
+#pragma unroll
+        for (int qb = 0; qb < PARTS; ++qb) mma_step(x[qb], Tl::frag(left, qb * 32, s, at), kv[s]);
       if (!second) {
         const float one = MODE == ONE ? by_distance[jw < i0 + ahead ? 0 : 2 * (far + PAD)] : 0.0f;
         const float* near = by_distance + (min(max(pos_k - ahead - i0 - 4 * half, -far), far + 60) + far + PAD);
