@@ -14,7 +14,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// (the low half of a flat address is the place in LDS; the plain cast would test it for null)
+// (the low half of a flat address is the place in LDS; the plain cast would test it for null.  The host's pass, whose
+// pointers are 64 bits, warns of the width.)
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"
 #define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(unsigned)(uintptr_t)(p))
 
 // row of the block that accumulator r of lane half h holds

@@ -338,6 +338,9 @@ static TokenPlan token_plan(int batch, int nq, int nk, int heads, int kv_heads) 
   const long busy = std::max((long)std::min(batch, nq), (long)i2r_cdiv(nq, 1 << p.shift)) * kv_heads * p.chunks;
   const long most = std::max(1L, (long)nk / std::max(batch, 1) / 256);
   p.splits = (int)std::max(1L, std::min({most, (2048 + busy - 1) / std::max(busy, 1L), 512L}));
+  // (many sequences without queries are workgroups too)
+  const long slots = ((long)(nq >> p.shift) + batch + 2) * kv_heads * p.chunks;
+  p.splits = (int)std::max(1L, std::min((long)p.splits, (1L << 22) / slots));
   return p;
 }
 

@@ -88,6 +88,8 @@ class RelativeBuckets:
         """The device's copy of `lut`, made once."""
         lut = self._on.get(device)
         if lut is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.I2RError("RelativeBuckets: first use on this device inside a stream capture; use them once before")
             lut = self._on[device] = self.lut.to(device)
         return lut
 
@@ -256,6 +258,8 @@ def packed_attention_fwd(q, k, v, seqs, bias=None, scale=None, out=None, save=Fa
         out = torch.empty((nq, heads, dim), dtype=q.dtype, device=dev)
     elif tuple(ops._chk(out, "out", q.dtype).shape) != (nq, heads, dim) or out.device != dev or out.data_ptr() % 16:
         raise ValueError(f"out: expected a 16-byte aligned ({nq}, {heads}, {dim}) tensor on {dev}")
+    elif any(out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() for t in (q, k, v)) and out.numel():
+        raise ValueError("out: shares its storage with q, k or v, which are read after the first rows are written")
     out32 = stats = None
     if save:
         out32 = out if dt == 0 else torch.empty((nq, heads, dim), dtype=torch.float32, device=dev)
@@ -325,8 +329,14 @@ def packed_attention(q, k, v, seqs, bias=None, scale=None, out=None):
     float32, float16 or bfloat16, dim a multiple of 8 up to 128.  Views (one projection's output split into q, k, v; a
     cache) are read in place where their rows are contiguous and 16-byte aligned, others are copied.  ``bias``: fp32
     (heads, num_buckets) table of the sequences' buckets.  ``scale``: dim ** -0.5 by default.  A query without keys gets
-    0; a key of score -inf counts as hidden.  Rows of q in no sequence come out 0 -- with ``out`` (inference only) they
-    are left as they were.  Differentiable in q, k, v and bias; the gradients' sums have a fixed order."""
+    0; a key of score -inf counts as hidden.  Rows of q in no sequence come out 0 -- with ``out`` (inference only, storage
+    of its own) they are left as they were.  Differentiable in q, k, v and bias; the gradients' sums have a fixed order.
+
+    Where a sequence has few queries (their mean number times the query heads that share a key / value head is at most
+    32) the keys are split over workgroups, as a token against its cache wants it: batches that mix prompts and single
+    tokens are faster in two calls.  A stream capture of forward and backward calls packed_attention_fwd and
+    packed_attention_bwd, or captures the whole training step; autograd's own graph of an earlier eager pass must not be
+    alive then (torch ends the process)."""
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v, bias)):
         if out is not None:
             raise ValueError("packed_attention: out= cannot be differentiated")

@@ -166,14 +166,14 @@ def test_rows_of_no_sequence(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
-@pytest.mark.parametrize("dim", [16, 64, 128])
-def test_hidden_values_are_never_used(dtype, dim):
+@pytest.mark.parametrize("dim,heads,kv", [(16, 2, 1), (64, 2, 1), (128, 2, 1), (64, 2, 2), (128, 2, 2), (96, 128, 64)])
+def test_hidden_values_are_never_used(dtype, dim, heads, kv):
     """Causal: NaN and infinities in a sequence's last key and value row reach its last query alone, forward and
     backward; the last query's own NaN gradient reaches what it sees, but no earlier row's dq."""
     import imageni2r_amd as i2r
     gen = torch.Generator(DEV).manual_seed(dim)
     lens = [70, 1, 129]
-    q, k, v, _, seqs, ref = _make(gen, dtype, dim, 2, 1, lens, causal=True)
+    q, k, v, _, seqs, ref = _make(gen, dtype, dim, heads, kv, lens, causal=True)
     clean = reference(q, k, v, dout=(dout := _rand(gen, *q.shape, dtype=dtype)), **ref)
     ends = [n - 1 for n in _cu(lens)[1:]]
     for bad_k, bad_v in ((math.nan, math.nan), (math.inf, -math.inf), (1.0, math.nan)):
@@ -192,7 +192,7 @@ def test_hidden_values_are_never_used(dtype, dim):
     # a later query's NaN does not reach the keys that it cannot see
     first = [_cu(lens)[0], _cu(lens)[2]]
     q2, dout2 = q.clone(), _rand(gen, *q.shape, dtype=dtype)
-    want = reference(q, k, v, dout=torch.where(torch.arange(len(q), device=DEV)[:, None, None] < 0, dout2, dout2), **ref)
+    want = reference(q, k, v, dout=dout2, **ref)
     q2[first], dout2b = math.nan, dout2.clone()
     dout2b[first] = math.nan
     got = _grads(q2, k, v, None, seqs, dout2b)
@@ -402,6 +402,87 @@ def test_only_the_gradients_that_are_asked_for():
         with pytest.raises(RuntimeError):
             torch.autograd.grad(torch.autograd.grad(i2r.packed_attention(*ops[:3], seqs, bias=ops[3]).float().sum(),
                                                     ops[at], create_graph=True)[0].float().sum(), ops[at])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("batch,longest", [(63, 9), (64, 9), (65, 130), (130, 40), (300, 5)])
+def test_many_sequences(dtype, batch, longest):
+    """More sequences than a wave has lanes, some of them empty."""
+    gen = torch.Generator(DEV).manual_seed(batch)
+    lens = torch.randint(0, longest + 1, (batch,), generator=gen, device=DEV).tolist()
+    _all(gen, *_make(gen, dtype, 16, 2, 1, lens, bias=(8, 20, True), causal=batch % 2 == 0))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,kv", [(24, 40, 1), (64, 64, 1), (128, 48, 1), (32, 66, 2), (96, 7, 1), (128, 128, 64),
+                                          (64, 96, 48)])
+def test_wide_groups_and_many_key_heads(dtype, dim, heads, kv):
+    """Groups of more heads than a tile has columns, tokens and prompts; enough key / value heads that none is split."""
+    gen = torch.Generator(DEV).manual_seed(heads)
+    _all(gen, *_make(gen, dtype, dim, heads, kv, [3, 90, 40], causal=True))
+    _all(gen, *_make(gen, dtype, dim, heads, kv, [1, 2, 0, 1], [70, 300, 5, 1], bias=(16, 50, False), causal=True))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [-0.7, 0.0, 0.3])
+@pytest.mark.parametrize("lens_q,lens_k", [([40, 70], None), ([1, 3], [900, 1300])])
+def test_scale(dtype, scale, lens_q, lens_k):
+    gen = torch.Generator(DEV).manual_seed(4)
+    _all(gen, *_make(gen, dtype, 40, 2, 2, lens_q, lens_k, causal=True), scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,kv", [(64, 4, 2), (128, 4, 4), (16, 6, 1)])
+@pytest.mark.parametrize("room", [64, 2000])
+def test_few_rows_with_gaps_and_hidden_values(dtype, dim, heads, kv, room):
+    """A few tokens a sequence against short and long (split) keys: rows of no sequence around and behind them, and NaN and
+    infinities in each sequence's last key, which only its last token sees."""
+    import imageni2r_amd as i2r
+    gen = torch.Generator(DEV).manual_seed(dim + room)
+    cu_q, n, fill = [2, 5, 5, 8], 11, [room, 7, room - 3]
+    q = _rand(gen, n, heads, dim, dtype=dtype)
+    k, v = (_rand(gen, 3 * room + 5, kv, dim, dtype=dtype) for _ in range(2))
+    cu_k = [room * b for b in range(4)]
+    seqs = i2r.PackedSequences(_i32(cu_q), _i32(cu_k), len_k=_i32(fill), causal=True)
+    dout = _rand(gen, n, heads, dim, dtype=dtype)
+    want = reference(q, k, v, cu_q, cu_k, fill, True, dout=dout)
+    last = [cu_k[b] + fill[b] - 1 for b in (0, 2)]
+    k[last], v[last] = math.nan, math.inf
+    ends, outside = [4, 7], [0, 1, 8, 9, 10]
+    seen = torch.ones(n, dtype=torch.bool, device=DEV)
+    seen[ends] = False
+    out = i2r.packed_attention(q, k, v, seqs)
+    check("out", out[seen], want["out"][0][seen], want["out"][1][seen])
+    assert bool((out[outside] == 0).all()) and bool(torch.isnan(out[ends].float()).any(-1).all())
+    mark = torch.full_like(q, 7.0)
+    i2r.packed_attention(q, k, v, seqs, out=mark)
+    assert bool((mark[outside] == 7).all()) and torch.equal(mark[[2, 3, 5, 6]], out[[2, 3, 5, 6]])
+    got = _grads(q, k, v, None, seqs, dout)
+    check("dq", got["dq"][seen], want["dq"][0][seen], want["dq"][1][seen])
+    assert bool((got["dq"][outside] == 0).all())
+
+
+@pytest.mark.parametrize("heads,kv", [(2, 2), (4, 1), (128, 64)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_fp16_gradients_beyond_the_lifted_range(heads, kv, dim):
+    """p and ds carry 2^12 in fp16: gradients so large that a lifted ds leaves the type's range, and so small that an
+    unlifted one would vanish."""
+    gen = torch.Generator(DEV).manual_seed(dim)
+    q, k, v, table, seqs, ref = _make(gen, F16, dim, heads, kv, [30, 65], bias=(8, 20, True))
+    for size in (40.0, 2e-3):
+        dout = _rand(gen, *q.shape, dtype=F16, size=size)
+        want = reference(q, k, v, dout=dout, **ref)
+        got = _grads(q, k, v, table, seqs, dout)
+        for name, w in want.items():
+            check(name, got[name], *w)
+
+
+def test_out_of_its_own():
+    import imageni2r_amd as i2r
+    q, k, v, _, seqs, _ = _make(torch.Generator(DEV).manual_seed(1), BF16, 64, 2, 2, [40], fused=True)
+    q = q.contiguous()
+    with pytest.raises(ValueError, match="storage"):
+        i2r.packed_attention(q, k, v, seqs, out=q)
 
 
 def test_no_rows():
