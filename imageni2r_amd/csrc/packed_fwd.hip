@@ -6,7 +6,7 @@
 template <typename T, int W>
 struct FwdShape {
   static constexpr int DP = Tile<T, W, 32>::DP;
-  static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 ? 32 : 64;
+  static constexpr int WAVES = 4, ROWS = 32 * WAVES, KEYS = sizeof(T) == 4 && W > 64 ? 32 : 64;
   typedef Tile<T, W, KEYS> Tl;
   static constexpr int MOST = W > 64 ? 2 : 4;
   static constexpr int BUFFER = 2 * Tl::BYTES + 256;  // k, v, positions
