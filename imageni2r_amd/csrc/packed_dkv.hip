@@ -1,4 +1,10 @@
 // Backward of packed-sequence attention on the matrix cores: dk and dv (packed_dq.hip has the other half).
+//
+// A key is a column, the queries of its group's heads pass by in tiles: both gradients of a key stay in one wave's
+// accumulators until the end, shared heads are summed there, and no addition is atomic.  Bound by matrix and vector
+// instructions that hardly overlap.  Measured (kernel traces, causal, bf16): eight documents of 2048 tokens, 32 heads of 128
+// over 8 784 us (701 TFLOP/s), 32 heads of 64 417 us (659); two documents of 4096 tokens, 32 heads of 128 over 8, with a
+// bias 647 us (849); 8192 tokens, 16 heads of 128 over 2, split over the group's heads, 566 us and 14 us of joining (949).
 #include "packed_tiles.h"
 
 // The lane's column of a sum, times `factor`, to its row; -> whether any of it is not finite.
@@ -73,8 +79,14 @@ struct DkvShape {
   static constexpr int WAVES = 4, COLS = 32 * WAVES / RG, ROWS = sizeof(T) == 4 ? 32 * RG : 64, SPAN = ROWS / RG;
   typedef Tile<T, W, ROWS> Tl;
   static constexpr int BUFFER = 2 * Tl::BYTES + 4 * 256;  // q, dout, delta, stats, positions
-  static constexpr int PER_SIMD = DP == 128 ? 1 : 2, UNROLL = DP == 128 || sizeof(T) == 4 ? 1 : 2;
+  static constexpr int UNROLL = DP == 128 || sizeof(T) == 4 ? 1 : 2;
   static constexpr bool APART = DP * sizeof(T) >= 256;
+  // The two that miss a third wave a SIMD (168 registers) by two are held to it: 64 wide in bf16, eight documents of 2048
+  // tokens, 32 heads 436 -> 370 us, 12 heads of 1024 both ways 79 -> 66 (but 4 x 512 18 -> 20); fp32, 32 wide with a bias,
+  // 32 x 384 121 -> 98.
+  static constexpr int per_simd(bool bias) {
+    return DP == 128 ? 1 : (sizeof(T) == 2 ? W == 64 && !bias : W == 32 && bias) ? 3 : 2;
+  }
   static constexpr int JOIN = 2 * COLS * (DP + 4) * 4;  // dk and dv of one group, where the tiles were
   static int lds(bool bias, int max_distance) {
     const int n = 2 * BUFFER + (bias ? table_places(max_distance) * 4 : 0);
@@ -83,7 +95,7 @@ struct DkvShape {
 };
 
 template <typename T, int W, bool BIAS>
-__global__ __launch_bounds__(256, (DkvShape<T, W>::PER_SIMD)) void pa_dkv_kernel(PaArgs a, long slots) {
+__global__ __launch_bounds__(256, (DkvShape<T, W>::per_simd(BIAS))) void pa_dkv_kernel(PaArgs a, long slots) {
   typedef DkvShape<T, W> S;
   typedef typename S::Tl Tl;
   extern __shared__ __align__(16) char lds[];
