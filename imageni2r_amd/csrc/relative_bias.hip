@@ -2,7 +2,8 @@
 //
 // Bound by writing, or reading, the dense tensor once.  A thread takes 8 neighbouring keys of a query: their bucket numbers
 // are looked up once for all heads (forward) and are mostly one and the same, so that the gradient's 8 terms are added in
-// registers and seldom reach the histogram.
+// registers and seldom reach the histogram.  Measured, 16 x 2048 x 2048 in bf16: forward 29 us (4.6 TB/s), gradient 41 + 4 us
+// (3.0 TB/s; torch's sum of a large tensor reads 4.0).
 #include "packed_common.h"
 
 struct BiasArgs {
