@@ -140,7 +140,6 @@ class PackedSequences:
             cu.append(cu[-1] + int(n))
         return cls(torch.tensor(cu, dtype=torch.int32, device=device), **kw)
 
-
     @classmethod
     def of_observed(cls, mask, buckets=None):
         """For series whose every step asks but whose observed steps alone answer: ``mask`` (B, L) bool, True where a step
@@ -151,17 +150,18 @@ class PackedSequences:
             raise TypeError(f"mask: expected a (B, L) bool tensor, got {tuple(mask.shape)} {mask.dtype}")
         B, L = mask.shape
         dev = mask.device
-        cu_q = torch.arange(0, (B + 1) * L, L, dtype=torch.int32, device=dev)
+        cu_q = torch.arange(B + 1, dtype=torch.int32, device=dev) * L
         cu_k = torch.zeros(B + 1, dtype=torch.int32, device=dev)
         torch.cumsum(mask.sum(1, dtype=torch.int32), 0, out=cu_k[1:])
         order = (~mask).reshape(-1).to(torch.uint8).argsort(stable=True)
         pos = dict(pos_q=torch.arange(L, dtype=torch.int32, device=dev).repeat(B),
-                   pos_k=(order % L).to(torch.int32)) if buckets is not None else {}
+                   pos_k=(order % max(L, 1)).to(torch.int32)) if buckets is not None else {}
         return cls(cu_q, cu_k, buckets=buckets, **pos), order
 
 
 def _rows(t, name, dtype, device):
-    """A (rows, heads, dim) operand: in place where its rows are contiguous and 16-byte aligned, else a copy."""
+    """A (rows, heads, dim) operand: in place where its rows are contiguous, 16-byte aligned and less than 2^22 elements
+    apart (heads may lie any way apart), else a copy."""
     if t.dim() != 3:
         raise ValueError(f"{name}: expected (rows, heads, dim), got {tuple(t.shape)}")
     if t.dtype != dtype:
@@ -170,7 +170,7 @@ def _rows(t, name, dtype, device):
         raise ValueError(f"{name}: on {t.device}, the sequences on {device}")
     s0, s1, s2 = t.stride()
     whole = 4 if dtype is torch.float32 else 8
-    if s2 != 1 or (s0 | s1) % whole or t.data_ptr() % 16 or s0 >= 1 << 22 or s1 >= 1 << 22:
+    if s2 != 1 or (s0 | s1) % whole or t.data_ptr() % 16 or s0 >= 1 << 22 or s1 >= 1 << 40:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -327,7 +327,8 @@ def packed_attention(q, k, v, seqs, bias=None, scale=None, out=None):
 
     q (rows, heads, dim); k, v (rows, kv_heads, dim), query head h reading key / value head h // (heads // kv_heads);
     float32, float16 or bfloat16, dim a multiple of 8 up to 128.  Views (one projection's output split into q, k, v; a
-    cache) are read in place where their rows are contiguous and 16-byte aligned, others are copied.  ``bias``: fp32
+    cache, token by token or head by head) are read in place where their rows are contiguous, 16-byte aligned and less than
+    2^22 elements apart, others are copied.  ``bias``: fp32
     (heads, num_buckets) table of the sequences' buckets.  ``scale``: dim ** -0.5 by default.  A query without keys gets
     0; a key of score -inf counts as hidden.  Rows of q in no sequence come out 0 -- with ``out`` (inference only, storage
     of its own) they are left as they were.  Differentiable in q, k, v and bias; the gradients' sums have a fixed order.

@@ -211,8 +211,8 @@ typedef struct i2r_packed_seqs {
 } i2r_packed_seqs;
 /* out_i = sum_j softmax_j(scale * <q_i, k_j> + table[h][bucket]) v_j for each query head h and its key / value head
  * h / (heads / kv_heads).  dtype: 0 fp32, 1 fp16, 2 bf16 (q, k, v, out alike); dim a multiple of 8 up to 128; each row of
- * q, k, v: `dim` contiguous elements, token and head strides in ELEMENTS, rows 16-byte aligned; out (nq, heads, dim)
- * contiguous.  A query that sees no key, or only scores of -inf, gets 0.  Hidden keys' values are never used, be they
+ * q, k, v: `dim` contiguous elements, token (below 2^22) and head strides in ELEMENTS, rows 16-byte aligned; out (nq,
+ * heads, dim) contiguous; below 2^30 rows; in the backward heads * dim below 2^22; ws 16-byte aligned.  A query that sees no key, or only scores of -inf, gets 0.  Hidden keys' values are never used, be they
  * NaN.  table: (heads, num_buckets) fp32 or NULL.  stats (2 * heads * nq floats: per row the softmax's reference exponent
  * and log2 of its sum) and out32 (out before its rounding; NULL for fp32) are what the backward reads; NULL when there is
  * none.  zero_outside: rows of no sequence are zeroed in out (0: left as they were).  ws: ws_bytes from the query (may be

@@ -525,3 +525,34 @@ def test_refusals():
             P(*args, **kw)
     with pytest.raises(ValueError):  # positions of another number of rows
         at(q, k, v, P(cu, buckets=seqs.buckets, pos_q=cu), bias=table)
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_cache_that_holds_head_after_head(dtype, rows):
+    """Heads 2^22 elements and more apart are read where they lie, in both directions and by the token kernel."""
+    import imageni2r_amd as i2r
+    from imageni2r_amd import packed
+    gen = torch.Generator(DEV).manual_seed(41)
+    room, dim, kv, heads, used = (1 << 15) + 8, 128, 2, 4, 700
+    cache = torch.zeros(2, kv, room, dim, dtype=dtype, device=DEV)
+    cache[:, :, :used] = _rand(gen, 2, kv, used, dim, dtype=dtype)
+    k, v = cache[0].transpose(0, 1), cache[1].transpose(0, 1)
+    assert k.stride(1) >= 1 << 22
+    assert packed._rows(k, "k", dtype, k.device).data_ptr() == k.data_ptr()
+    q, dout = _rand(gen, rows, heads, dim, dtype=dtype), _rand(gen, rows, heads, dim, dtype=dtype)
+    seqs = i2r.PackedSequences(_i32([0, rows]), _i32([0, room]), len_k=_i32([used]), causal=True)
+    got = _grads(q, k, v, None, seqs, dout)
+    want = _grads(q, k.contiguous(), v.contiguous(), None, seqs, dout)
+    for name in got:
+        assert torch.equal(got[name], want[name]), name
+    with torch.no_grad():
+        assert torch.equal(i2r.packed_attention(q, k, v, seqs), i2r.packed_attention(q, k.contiguous(), v.contiguous(), seqs))
+
+
+def test_observed_steps_of_series_without_steps():
+    import imageni2r_amd as i2r
+    seqs, order = i2r.PackedSequences.of_observed(torch.zeros(3, 0, dtype=torch.bool, device=DEV), i2r.RelativeBuckets())
+    assert order.numel() == 0 and seqs.cu_q.tolist() == [0, 0, 0, 0] == seqs.cu_k.tolist()
+    q = torch.zeros(0, 2, 8, device=DEV)
+    assert i2r.packed_attention(q, q, q, seqs, bias=torch.zeros(2, 32, device=DEV)).shape == (0, 2, 8)

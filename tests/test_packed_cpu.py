@@ -99,3 +99,12 @@ def test_sizes_of_workspaces_take_any_sizes():
     for n in (0, 1, 7, 100000):
         assert _lib.query("i2r_packed_attention_fwd_ws_bytes", 2, 3, n, n, 8, 2, 64) >= 0
         assert _lib.query("i2r_packed_attention_bwd_ws_bytes", 2, 3, n, n, 8, 2, 64, 32) >= 0
+
+
+def test_c_refuses_tokens_too_far_apart():
+    from imageni2r_amd import _lib
+    for i in (0, 2, 4):
+        strides = [32, 16] * 3
+        strides[i] = 1 << 22
+        with pytest.raises(_lib.I2RError, match="below 2\\^22"):
+            _fwd(strides=strides)
