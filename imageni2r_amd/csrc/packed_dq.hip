@@ -1,7 +1,7 @@
 // Backward of packed-sequence attention on the matrix cores: dq and the table's gradient.
 //
-// The backward is two kernels, both recomputing the scores: dq (a query a column, keys pass by) and dk / dv (a key a column, the queries of
-// all heads of its group pass by).  Seven products where five would do with dq added up atomically -- but no float is ever
+// The backward is two kernels, both recomputing the scores: dq (a query a column, keys pass by) and dk / dv (a key a
+// column, the queries of all heads of its group pass by).  Seven products where five would do with dq added up atomically -- but no float is ever
 // added in an order that could change, and nothing but the outputs is written.
 //
 // Bound as the forward is, by matrix and vector instructions that hardly overlap; with a bias at 128 the histogram leaves
@@ -42,8 +42,8 @@ struct DqShape {
   }
 };
 
-// dq of 32 queries a wave, delta = <dout, out> and the two stats' sum on the way for the other kernel, and ds summed by bucket: each lane its own column of a histogram
-// in LDS, so that no two lanes add to one word.
+// dq of 32 queries a wave, delta = <dout, out> and the two stats' sum on the way for the other kernel, and ds summed by
+// bucket: each lane its own column of a histogram in LDS, so that no two lanes add to one word.
 template <typename T, int W, bool BIAS>
 __global__ __launch_bounds__(256, (DqShape<T, W>::PER_SIMD)) void pa_dq_kernel(PaArgs a, long slots) {
   typedef DqShape<T, W> S;

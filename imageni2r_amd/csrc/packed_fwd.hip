@@ -6,9 +6,9 @@
 // per query (fp32) and the output is scaled when the exponent moves.
 //
 // Bound by the issue of matrix and vector instructions together: the two hardly overlap here (16384 tokens, 128 wide:
-// matrix pipes busy 42 % of the time, vector pipes 45 %), and per 64 keys a wave needs 32 products of 32 cycles, 32
+// matrix pipes busy 50 % of the time, vector pipes 47 %), and per 64 keys a wave needs 32 products of 32 cycles, 32
 // exponentials of 16 and some 120 other instructions of 4.  Measured: 16384 tokens, 16 heads of 128 over 2, causal, bf16
-// 1086 us (1013 TFLOP/s; a library product of 8192^3 reaches 1105); lengths up to 1999, 12 heads of 80, both directions,
+// 1086 to 1108 us (up to 1013 TFLOP/s; a library product of 8192^3 reaches 1105); lengths up to 1999, 12 heads of 80, both directions,
 // fp16 113 us (558); 16 prompts of up to 1024, 16 heads of 64 over 4, with a bias 49 us (401: at 64 wide the exponentials
 // weigh twice as much, and short sequences leave the start and end of a workgroup in view).
 //
