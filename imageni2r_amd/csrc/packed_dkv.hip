@@ -82,8 +82,8 @@ struct DkvShape {
   static constexpr int UNROLL = DP == 128 || sizeof(T) == 4 ? 1 : 2;
   static constexpr bool APART = DP * sizeof(T) >= 256;
   // The two that miss a third wave a SIMD (168 registers) by two are held to it: 64 wide in bf16, eight documents of 2048
-  // tokens, 32 heads 436 -> 370 us, 12 heads of 1024 both ways 79 -> 66 (but 4 x 512 18 -> 20); fp32, 32 wide with a bias,
-  // 32 x 384 121 -> 98.
+  // tokens, 32 heads 445 -> 385 us, 12 heads of 1024 both ways 81 -> 67; fp32, 32 wide with a bias, 32 x 384 122 -> 98.
+  // (Where two workgroups a CU hold all there is it gains nothing: fp32 of 32 with a bias, 4 x 1024, 154 -> 157.)
   static constexpr int per_simd(bool bias) {
     return DP == 128 ? 1 : (sizeof(T) == 2 ? W == 64 && !bias : W == 32 && bias) ? 3 : 2;
   }
@@ -491,9 +491,16 @@ template <typename T, int W>
 static bool launch_dkv(const PaArgs& a, hipStream_t st) {
   typedef DkvShape<T, W> S;
   const long slots = a.nk / S::COLS + a.s.batch + 2;
+  // Two workgroups a CU where that holds them all, by as much LDS as lets no third in: it would stand on some CUs while others
+  // have one.  4 x 1024 tokens, 16 heads over 8, both ways, with against without: fp32 of 32 with a bias 157 us, 218; bf16 of
+  // 64 50, 55.
+  const int least = a.nk / S::COLS * (long)a.kv_heads * a.parts <= 512 ? 56 << 10 : 0;
   if (a.table)
-    PA_LAUNCH((pa_dkv_kernel<T, W, true>), slots, a.kv_heads * a.parts, S::lds(true, a.s.max_distance), S::lds(true, PA_MAX_DISTANCE))
-  else PA_LAUNCH((pa_dkv_kernel<T, W, false>), slots, a.kv_heads * a.parts, S::lds(false, 0), S::lds(false, 0))
+    PA_LAUNCH((pa_dkv_kernel<T, W, true>), slots, a.kv_heads * a.parts, std::max(least, S::lds(true, a.s.max_distance)),
+              std::max(56 << 10, S::lds(true, PA_MAX_DISTANCE)))
+  else
+    PA_LAUNCH((pa_dkv_kernel<T, W, false>), slots, a.kv_heads * a.parts, std::max(least, S::lds(false, 0)),
+              std::max(56 << 10, S::lds(false, 0)))
   return true;
 }
 
