@@ -225,20 +225,51 @@ __global__ __launch_bounds__(256, (DqShape<T, W>::PER_SIMD)) void pa_dq_kernel(P
         }
         if (valid && d < a.dim) *(t4*)((T*)a.dq + to + d) = y;
       }
-  if (sums) {
-    __syncthreads();
-    const float* all = (const float*)(by_distance + table_places(far));
-    for (int c = wave; c < nb; c += S::WAVES) {
-      float s = 0.0f;
-      for (int v = 0; v < S::WAVES; ++v) s += all[(v * nb + c) * 64 + lane];
-      s = wave_sum(s);
-      if (lane == 0) a.part[(slot * a.heads + h) * nb + c] = s * Lift<T>::DOWN;
-    }
-  }
-  // a hidden pair's 0 times NaN, or a lifted ds beyond fp16: pair by pair
+  // A hidden pair's 0 times NaN, or a lifted ds beyond fp16: those queries are done again, pair by pair.  What no query of the
+  // tile sees reaches the histogram too, where its score is -inf or the column holds no query (and a made-up place, 0): if a
+  // bucket's sum comes out not finite, the columns that are to blame are emptied, and their queries' ds added pair by pair.
+  // (A test of each pair's score instead would be two instructions more in the loop over the keys.)
   const unsigned long long again = __ballot(valid && !(finite == 0.0f));
-  for (unsigned rows = (unsigned)again | (unsigned)(again >> 32); rows; rows &= rows - 1)
-    pa_row_dq<T>(a, w, iw + __ffs(rows) - 1, h);
+  unsigned rows = (unsigned)again | (unsigned)(again >> 32), by_bucket = 0;
+  int own = lane;
+  asm volatile("" : "+v"(own));  // (keeps the columns' places below out of the registers above: 64 wide they would be 169)
+#pragma unroll 1
+  for (bool first = true;; first = false) {
+    bool done = true;
+    if (sums) {
+      __syncthreads();
+      const float* all = (const float*)(by_distance + table_places(far));
+      float off = 0.0f;
+      for (int c = wave; c < nb; c += S::WAVES) {
+        float s = 0.0f;
+        for (int v = 0; v < S::WAVES; ++v) s += all[(v * nb + c) * 64 + own];
+        s = wave_sum(s);
+        off = fmaf(s, 0.0f, off);
+        if (own == 0) a.part[(slot * a.heads + h) * nb + c] = s * Lift<T>::DOWN;
+      }
+      if (first) {
+        int* marks = (int*)lds;  // (the tiles are read)
+        if (own == 0) marks[wave] = off == 0.0f;
+        __syncthreads();
+        for (int v = 0; v < S::WAVES; ++v) done &= marks[v] != 0;
+        if (!done) {
+          off = 0.0f;
+          for (int c = 0; c < nb; ++c) off = fmaf(hist[c * 64 + own], 0.0f, off);
+          const unsigned long long bad = __ballot(!(off == 0.0f)), live = __ballot(valid);
+          by_bucket = (unsigned)bad | (unsigned)(bad >> 32);
+          if (by_bucket >> (own & 31) & 1)
+            for (int c = 0; c < nb; ++c) hist[c * 64 + own] = 0.0f;
+          by_bucket &= (unsigned)live;
+        }
+      }
+    }
+    for (rows |= by_bucket; rows; rows &= rows - 1) {
+      const int c = __ffs(rows) - 1;
+      pa_row_dq<T>(a, w, iw + c, h, by_bucket >> c & 1 ? hist + own : nullptr);
+    }
+    by_bucket = 0;
+    if (done) break;
+  }
 }
 
 #define PA_LAUNCH(KERNEL, SLOTS, HEADS, LDS, MOST)                                                         \

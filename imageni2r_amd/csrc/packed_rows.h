@@ -149,9 +149,9 @@ __device__ __forceinline__ void pa_pair(const PaArgs& a, float x, long row, int 
   ds = p * (pa_dot(doi, vj, a.dim) - a.delta[at]);
 }
 
-// dq of query i, head h.
+// dq of query i, head h; with `hist` (a lane's column of it, 64 apart) its ds by bucket too, each lane's keys to its own column.
 template <typename T>
-__device__ __forceinline__ void pa_row_dq(const PaArgs& a, const PaSeq& w, int i, int h) {
+__device__ __forceinline__ void pa_row_dq(const PaArgs& a, const PaSeq& w, int i, int h, float* hist = nullptr) {
   const int lane = threadIdx.x & 63, g = h / (a.heads / a.kv_heads);
   const long row = w.q0 + i, at = (row * a.heads + h) * a.dim;
   const T* qi = (const T*)a.q + row * a.q_row + h * a.q_head;
@@ -165,7 +165,10 @@ __device__ __forceinline__ void pa_row_dq(const PaArgs& a, const PaSeq& w, int i
     float x = -INFINITY, p = 0.0f, ds = 0.0f;
     if (j < seen) {
       x = pa_score(a, w, h, qi, (const T*)a.k + (long)(w.k0 + j) * a.k_row + g * a.k_head, pos_q, j, bucket);
-      if (!(x == -INFINITY)) pa_pair(a, x, row, h, doi, (const T*)a.v + (long)(w.k0 + j) * a.v_row + g * a.v_head, p, ds);
+      if (!(x == -INFINITY)) {
+        pa_pair(a, x, row, h, doi, (const T*)a.v + (long)(w.k0 + j) * a.v_row + g * a.v_head, p, ds);
+        if (hist) hist[bucket * 64] += ds / Lift<T>::DOWN;
+      }
     }
     for (unsigned long long open = __ballot(!(x == -INFINITY)); open; open &= open - 1) {
       const int t = __ffsll(open) - 1;
