@@ -189,7 +189,10 @@ __global__ __launch_bounds__((64 * TokenShape<T, W>::WAVES), (TokenShape<T, W>::
   for (int v = 0; v < S::WAVES; ++v) top = fmaxf(top, wm[v * 32 + col]);
 #pragma unroll
   for (int v = 0; v < S::WAVES; ++v)
-    sum += wm[v * 32 + col] == -INFINITY ? 0.0f : wl[v * 32 + col] * __builtin_amdgcn_exp2f(wm[v * 32 + col] - top);
+    sum += wl[v * 32 + col] * (wm[v * 32 + col] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[v * 32 + col] - top));
+  // The largest of scores that are all NaN is -inf, as of none: that some were is left in the sum, and has to reach the join of
+  // the splits.
+  if (top == -INFINITY && sum != sum) top = NAN;
   const float fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
   float* mine = (float*)tiles;
 #pragma unroll
