@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, FwdSh
         for (int r = 0; r < 16; ++r) o[b][r] *= fall;
       m = mn;
     }
-    const float ref = m == -INFINITY ? 0.0f : m;
+    const float ref = m == -INFINITY ? 0.0f : m - Lift<T>::FWD_LOG2;
 #pragma unroll
     for (int kb = 0; kb < BLOCKS; ++kb) {
 #pragma unroll
@@ -148,7 +148,8 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, FwdSh
       }
       // Rounding the probabilities to the type puts each off by at most half a step, independently: as much as rounding
       // the output once more.  The table's gradient is fp32, and delta = <dout, out> enters it: with a bias to train
-      // what the rounding took away is multiplied too, until 22 bits (fp16) or 24 (bf16) of each have been.
+      // what the rounding took away is multiplied too, until 22 bits (fp16, or 2^-32 where that is more) or 24 (bf16) of each
+      // have been.
       Probs<T> p;
       if constexpr (BIAS && SAVE && sizeof(T) == 2) {
 #pragma unroll
@@ -198,6 +199,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, FwdSh
   }
 
   l += other_half(l);
+  m -= Lift<T>::FWD_LOG2;  // what l is relative to (of a score of 2^27 the 7 is rounded away, here as there)
   const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
   float finite = l * 0.0f;
   const long to = ((long)(w.q0 + i) * a.heads + h) * a.dim;

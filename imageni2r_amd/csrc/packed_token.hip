@@ -153,7 +153,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, W>::WAVES), (TokenShape<T, W>::
         for (int r = 0; r < 16; ++r) o[t][r] *= fall;
       m = mn;
     }
-    const float ref = m == -INFINITY ? 0.0f : m;
+    const float ref = m == -INFINITY ? 0.0f : m - Lift<T>::FWD_LOG2;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = __builtin_amdgcn_exp2f(BIAS ? x[r] - ref : fmaf(x[r], sc, -ref));
@@ -176,6 +176,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, W>::WAVES), (TokenShape<T, W>::
     }
   }
   l += other_half(l);
+  m -= Lift<T>::FWD_LOG2;  // what l is relative to (of a score of 2^27 the 7 is rounded away, here as there)
 
   // join the waves
   float* wm = small;                    // [wave][col]
