@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
@@ -304,6 +305,18 @@ def packed_attention_bwd(q, k, v, seqs, bias, out32, stats, dout, scale=None, ne
     return dq, dk, dv, dbias
 
 
+def _differentiated(*tensors):
+    """Whether autograd has to see the call: an input that asks for a gradient, or one that carries a tangent -- which the
+    functions below have no derivative for, so that torch refuses it."""
+    dual = getattr(forward_ad, "_current_level", 0) >= 0  # without an open dual level there are no tangents
+    if dual or torch.is_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and (t.requires_grad and torch.is_grad_enabled() or
+                                                dual and forward_ad.unpack_dual(t).tangent is not None):
+                return True
+    return False
+
+
 class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, seqs, scale):
@@ -331,14 +344,15 @@ def packed_attention(q, k, v, seqs, bias=None, scale=None, out=None):
     2^22 elements apart, others are copied.  ``bias``: fp32
     (heads, num_buckets) table of the sequences' buckets.  ``scale``: dim ** -0.5 by default.  A query without keys gets
     0; a key of score -inf counts as hidden.  Rows of q in no sequence come out 0 -- with ``out`` (inference only, storage
-    of its own) they are left as they were.  Differentiable in q, k, v and bias; the gradients' sums have a fixed order.
+    of its own) they are left as they were.  Differentiable in q, k, v and bias, backward and once (tangents are refused); the
+    gradients' sums have a fixed order.
 
     Where a sequence has few queries (their mean number times the query heads that share a key / value head is at most
     32) the keys are split over workgroups, as a token against its cache wants it: batches that mix prompts and single
     tokens are faster in two calls.  A stream capture of forward and backward calls packed_attention_fwd and
     packed_attention_bwd, or captures the whole training step; autograd's own graph of an earlier eager pass must not be
     alive then (torch ends the process)."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v, bias)):
+    if _differentiated(q, k, v, bias):
         if out is not None:
             raise ValueError("packed_attention: out= cannot be differentiated")
         return PackedAttentionFn.apply(q, k, v, bias, seqs, scale)
@@ -402,7 +416,7 @@ class RelativeBiasFn(torch.autograd.Function):
 def relative_bias(table, buckets, q_len, k_len, pos_q=None, pos_k=None, dtype=torch.float32):
     """The bias of ``table`` (heads, num_buckets) fp32 as a dense (heads, q_len, k_len) tensor of ``dtype``, for an
     attention that takes an additive mask.  Positions: int32 vectors, or None: key j at j, query i at i + k_len - q_len.
-    Differentiable in ``table``; the gradient's sums have a fixed order."""
-    if torch.is_grad_enabled() and isinstance(table, torch.Tensor) and table.requires_grad:
+    Differentiable in ``table``, backward and once; the gradient's sums have a fixed order."""
+    if _differentiated(table):
         return RelativeBiasFn.apply(table, buckets, q_len, k_len, pos_q, pos_k, dtype)
     return relative_bias_fwd(table, buckets, q_len, k_len, pos_q, pos_k, dtype)
