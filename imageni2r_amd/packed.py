@@ -105,7 +105,8 @@ class PackedSequences:
     ``pos_q``), or without them by j and i + Lk - Lq.
 
     All arrays are int32 vectors on the HIP device, read by the kernels when they run: an object stays valid when their
-    values change (a cache that grows, a replayed graph) -- between a forward and its backward they must not.  Nothing
+    values change (a cache that grows, a replayed graph: ``seqs.len_k.copy_(...)``) -- between a forward and its backward
+    they must not.  The attributes themselves are fixed: the kernels have the arrays' addresses from the start.  Nothing
     checks the values on the host: the kernels clamp them to the tensors they are used with, and sequences have to
     ascend."""
 
@@ -132,6 +133,14 @@ class PackedSequences:
         self._c = _Seqs(*ptr, batch, int(self.causal), buckets.num_buckets if buckets else 0,
                         buckets.max_distance if buckets else 0)
         self._ref = ctypes.byref(self._c)
+
+    def __setattr__(self, name, value):
+        if self.__dict__.get(name, value) is not value:  # (len_k += 1 sets the array that it wrote into)
+            raise AttributeError(f"PackedSequences.{name} is fixed: write into the array (copy_), or make another object")
+        super().__setattr__(name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError(f"PackedSequences.{name} is fixed")
 
     @classmethod
     def from_lengths(cls, lengths, device="cuda", **kw):
