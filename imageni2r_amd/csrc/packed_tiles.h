@@ -17,6 +17,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // (the low half of a flat address is the place in LDS; the plain cast would test it for null.  The host's pass, whose
 // pointers are 64 bits, warns of the width.)
 #pragma clang diagnostic ignored "-Wint-to-pointer-cast"
+// (m0, where a load to LDS finds its place, is a register that the compiler keeps for itself: it obeys the clobber, and warns)
+#pragma clang diagnostic ignored "-Winline-asm"
 #define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(unsigned)(uintptr_t)(p))
 
 // row of the block that accumulator r of lane half h holds
@@ -198,7 +200,7 @@ struct Loader {
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    :
                    : "s"(to + i * WAVES * 1024), "v"(offset[i]), "s"(rs)
-                   : "memory");
+                   : "memory", "m0");
   }
 };
 
@@ -241,7 +243,7 @@ __device__ __forceinline__ void load_words(void* to, const void* from, int first
   asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(lds), "v"((int)threadIdx.x * 4), "s"(rs)
-               : "memory");
+               : "memory", "m0");
 }
 
 // Where a tile's bias comes from: there is none; all distances lie beyond max_distance on one side; places in the sequence;
