@@ -97,8 +97,10 @@ extern "C" int i2r_packed_attention_fwd(const i2r_packed_seqs* seqs, const void*
 
 static long q_slots(int nq, int batch) { return (nq >> 7) + batch + 2; }
 
-// A key / value head's query heads go to several workgroups, whose sums are joined, where the keys alone make fewer
-// workgroups than there are CUs: 8192 tokens, 16 heads of 128 over 2: dk and dv in 580 us instead of 2116.
+// A key / value head's query heads go to several workgroups, whose sums are joined, where the keys alone are too few: below 256
+// blocks of 128 keys, one for each CU, or two of the workgroups of 64 that most widths have.  Split against whole: 8192 tokens,
+// 16 heads over 2 (130 blocks), of 128 596 us, 2027; of 64 356, 1111; 6000 tokens, 16 heads of 64 over 4 (188) 252, 418; 2 x
+// 1024, over 8 (144) 39.5, 45.7; fp32 of 64, 4096 tokens, over 4 (132) 598, 1571.
 static int dkv_parts(int batch, int nk, int heads, int kv_heads) {
   const long busy = ((long)nk / 128 + batch) * kv_heads;
   return busy >= 256 ? 1 : (int)std::min((long)heads / kv_heads, (512 + busy - 1) / busy);

@@ -40,7 +40,8 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
 
 // fp16 holds no probability below 6e-8 and few digits below 6e-5: there p and ds carry 2^12 in the backward, taken out at the
 // end, and p 2^7 in the forward, where it may be 2^8 before the reference exponent moves (2^15 of the type's 2^16).  Each is
-// then rounded by at most 2^-25 / 2^7 = 2^-32, and what many small ones are together is not lost.
+// then rounded by at most 2^-25 / 2^7 = 2^-32, and what many small ones are together is not lost.  (A ds of 16 and more leaves
+// the type with its 2^12: those rows are done again pair by pair, in fp32, and off the matrix cores.)
 template <typename T>
 struct Lift {
   static constexpr float LOG2 = sizeof(T) == 2 && __is_same(T, f16_t) ? 12.0f : 0.0f;

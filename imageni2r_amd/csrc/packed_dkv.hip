@@ -1,10 +1,15 @@
 // Backward of packed-sequence attention on the matrix cores: dk and dv (packed_dq.hip has the other half).
 //
 // A key is a column, the queries of its group's heads pass by in tiles: both gradients of a key stay in one wave's
-// accumulators until the end, shared heads are summed there, and no addition is atomic.  Bound by matrix and vector
-// instructions that hardly overlap.  Measured (kernel traces, causal, bf16): eight documents of 2048 tokens, 32 heads of 128
-// over 8 784 us (701 TFLOP/s), 32 heads of 64 417 us (659); two documents of 4096 tokens, 32 heads of 128 over 8, with a
-// bias 647 us (849); 8192 tokens, 16 heads of 128 over 2, split over the group's heads, 566 us and 14 us of joining (949).
+// accumulators until the end, shared heads are summed there, and no addition is atomic.
+//
+// Bound by neither kind of instruction alone (counters): 128 wide, two documents of 4096 tokens, 32 heads over 8, the matrix
+// pipes are busy 29 % of the time, the vector pipes 20 %, and waves wait for half of theirs: for each other (two barriers a
+// tile) and at the end, for the longest workgroups; 64 wide with a bias, eight documents of up to 2048, 16 % and 28 %, with one
+// wave a SIMD on average, where two fit; fp32, 8 wide, 42 % and 25 %.  Measured (kernel traces, causal, bf16): eight documents of
+// 2048 tokens, 32 heads of 128 over 8 795 us (691 TFLOP/s), 32 heads of 64 410 us (670); two documents of 4096 tokens, 32
+// heads of 128 over 8, with a bias 678 us (810); 8192 tokens, 16 heads of 128 over 2, split over the group's heads, 621 us and
+// 15 us of joining (865).
 #include "packed_tiles.h"
 
 // The lane's column of a sum, times `factor`, to its row; -> whether any of it is not finite.
@@ -81,9 +86,12 @@ struct DkvShape {
   static constexpr int BUFFER = 2 * Tl::BYTES + 4 * 256;  // q, dout, delta, stats, positions
   static constexpr int UNROLL = DP == 128 || sizeof(T) == 4 ? 1 : 2;
   static constexpr bool APART = DP * sizeof(T) >= 256;
-  // The two that miss a third wave a SIMD (168 registers) by two are held to it: 64 wide in bf16, eight documents of 2048
-  // tokens, 32 heads 445 -> 385 us, 12 heads of 1024 both ways 81 -> 67; fp32, 32 wide with a bias, 32 x 384 122 -> 98.
-  // (Where two workgroups a CU hold all there is it gains nothing: fp32 of 32 with a bias, 4 x 1024, 154 -> 157.)
+  // The two that miss a third wave a SIMD (168 registers) by two are held to it.  In turn with dq, two waves against three: 64
+  // wide in bf16, eight documents of 2048 tokens, 32 heads 424 -> 359 us (a kernel trace has 410 for the latter), 16 over 4
+  // 77 -> 67, 12 heads of 1024 both ways 79 -> 66; fp32, 32 wide with a bias, 32 x 384 121 -> 97.  It loses where the
+  // grid is two rounds of two workgroups a CU, of three a whole round and a third of one: 4096 tokens, 16 heads of 64 over 4
+  // (1024 workgroups), 108 -> 117.  (Where two a CU hold all there is it gains nothing: fp32 of 32 with a bias, 4 x 1024,
+  // 154 -> 157.)
   static constexpr int per_simd(bool bias) {
     return DP == 128 ? 1 : (sizeof(T) == 2 ? W == 64 && !bias : W == 32 && bias) ? 3 : 2;
   }

@@ -4,10 +4,12 @@
 // column, the queries of all heads of its group pass by).  Seven products where five would do with dq added up atomically -- but no float is ever
 // added in an order that could change, and nothing but the outputs is written.
 //
-// Bound as the forward is, by matrix and vector instructions that hardly overlap; with a bias at 128 the histogram leaves
-// room for one workgroup a CU.  Measured (kernel traces, causal, bf16): eight documents of 2048 tokens, 32 heads of 128 over
-// 8 508 us (811 TFLOP/s), 32 heads of 64 295 us (700); two documents of 4096, 32 heads of 128 over 8, with a bias and the
-// table's gradient 703 us (586).
+// Bound by matrix and vector instructions, and by what keeps two waves a SIMD from filling each other's gaps (counters: 128
+// wide, two documents of 4096 tokens, matrix pipes busy 37 % of the time, vector pipes 30 %; 64 wide with a bias, eight of up to
+// 2048, 15 % and 39 %; fp32, 8 wide, bias by times, 25 % and 29 %); with a bias at 128 the histogram leaves room for one
+// workgroup a CU.  Measured (events, causal, bf16): eight documents of 2048 tokens, 32 heads of 128 over 8 493 us (837
+// TFLOP/s), 32 heads of 64 266 us (776); two documents of 4096, 32 heads of 128 over 8, with a bias and the table's gradient
+// 733 us (562).
 #include "packed_tiles.h"
 
 // Adds four keys' ds to the lane's column of the histogram, those of one bucket first: neighbours mostly share one, and a

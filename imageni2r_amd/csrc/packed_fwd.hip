@@ -5,12 +5,14 @@
 // this one is worked on (two LDS buffers, one barrier a tile).  One pass: the softmax's reference exponent and sum are kept
 // per query (fp32) and the output is scaled when the exponent moves.
 //
-// Bound by the issue of matrix and vector instructions together: the two hardly overlap here (16384 tokens, 128 wide:
-// matrix pipes busy 50 % of the time, vector pipes 47 %), and per 64 keys a wave needs 32 products of 32 cycles, 32
-// exponentials of 16 and some 120 other instructions of 4.  Measured: 16384 tokens, 16 heads of 128 over 2, causal, bf16
-// 1086 to 1108 us (up to 1013 TFLOP/s; a library product of 8192^3 reaches 1105); lengths up to 1999, 12 heads of 80, both directions,
-// fp16 113 us (558); 16 prompts of up to 1024, 16 heads of 64 over 4, with a bias 49 us (401: at 64 wide the exponentials
-// weigh twice as much, and short sequences leave the start and end of a workgroup in view).
+// Long sequences are bound by the issue of matrix and vector instructions together: the two hardly overlap there (16384 tokens,
+// 128 wide: matrix pipes busy 50 % of the time, vector pipes 47 %), and per 64 keys a wave needs 32 products of 32 cycles, 32
+// exponentials of 16 and some 120 other instructions of 4.  Short ones leave the start and end of a workgroup, and uneven
+// workgroups, in view: 16 prompts of up to 1024, 64 wide with a bias, 15 % and 41 % (the exponentials weigh twice as much at 64),
+// 1.6 waves a SIMD where two and more fit; sequences up to 1999, 80 wide, 27 % and 35 %; fp32, 8 wide, bias by times, 28 % and
+// 22 %.  Measured, on several cards: 16384 tokens, 16 heads of 128 over 2, causal, bf16 1027 to 1108 us (up to 1071 TFLOP/s; a
+// library product of 8192^3 reaches 1105); lengths up to 1999, 12 heads of 80, both directions, fp16 113 to 121 us (558); 16
+// prompts of up to 1024, 16 heads of 64 over 4, with a bias 49 to 55 us (401).
 //
 // 32 queries a wave: 64 would halve the LDS reads, but leave one wave a SIMD.  Tiles of 64 keys (fp32 at 128: 32) keep two
 // workgroups' buffers in 160 KB.

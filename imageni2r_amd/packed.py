@@ -358,9 +358,11 @@ def packed_attention(q, k, v, seqs, bias=None, scale=None, out=None):
 
     Where a sequence has few queries (their mean number times the query heads that share a key / value head is at most
     32) the keys are split over workgroups, as a token against its cache wants it: batches that mix prompts and single
-    tokens are faster in two calls.  A stream capture of forward and backward calls packed_attention_fwd and
-    packed_attention_bwd, or captures the whole training step; autograd's own graph of an earlier eager pass must not be
-    alive then (torch ends the process)."""
+    tokens are faster in two calls.  In fp16 a score's gradient of 16 and more (from an output gradient that was scaled
+    up) takes its rows off the matrix cores, at 50 times the time and more; bf16 has no such limit.
+
+    A stream capture of forward and backward calls packed_attention_fwd and packed_attention_bwd, or captures the whole
+    training step; autograd's own graph of an earlier eager pass must not be alive then (torch ends the process)."""
     if _differentiated(q, k, v, bias):
         if out is not None:
             raise ValueError("packed_attention: out= cannot be differentiated")
