@@ -65,3 +65,29 @@ def test_equal_scores_of_any_size(dtype, rows, keys, size, sign, bias):
     leaf = table.requires_grad_(True) if bias else q.requires_grad_(True)  # (what a backward pass needs is kept: another form)
     got = i2r.packed_attention(q, k, v, seqs, bias=table, scale=sign * size / 8)
     assert leaf.requires_grad and bool(((got.detach().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("rows,keys,heads,kv", [(1, 2000, 4, 2), (3, 40, 4, 4), (90, 300, 4, 1)])
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("lowest", ["all", "far", "near"])
+def test_fp16_tables_of_the_lowest_value(rows, keys, heads, kv, dim, lowest):
+    """Buckets of the type's lowest value in fp16, where the exponent that 2^7 is taken from has no place left for it: rows that
+    have nothing else weigh their keys alike, others leave those keys out; with gradients."""
+    import imageni2r_amd as i2r
+    from tests.packed_reference import check, reference
+    gen = torch.Generator(DEV).manual_seed(dim + rows)
+    q, dout = (torch.randn(rows, heads, dim, generator=gen, device=DEV).half() for _ in range(2))
+    k, v = (torch.randn(keys, kv, dim, generator=gen, device=DEV).half() for _ in range(2))
+    buckets = i2r.RelativeBuckets(16, 40, False)
+    table = torch.randn(heads, 16, generator=gen, device=DEV)
+    table[:, {"all": slice(None), "far": slice(15, 16), "near": slice(0, 15)}[lowest]] = torch.finfo(torch.float32).min
+    seqs = i2r.PackedSequences(torch.tensor([0, rows], dtype=torch.int32, device=DEV),
+                               torch.tensor([0, keys], dtype=torch.int32, device=DEV), causal=True, buckets=buckets)
+    want = reference(q, k, v, [0, rows], [0, keys], causal=True, table=table, buckets=buckets, dout=dout)
+    with torch.no_grad():
+        check("out, inference", i2r.packed_attention(q, k, v, seqs, bias=table), *want["out"])
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v, table)]
+    out = i2r.packed_attention(*leaves[:3], seqs, bias=leaves[3])
+    got = dict(zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(),) + torch.autograd.grad(out, leaves, dout)))
+    for name, w in want.items():
+        check(name, got[name], *w)
